@@ -310,7 +310,7 @@ def _attend(s):
     rows = s['q'].shape[0]
     lse = _packed(torch.where(lse == -math.inf, 0.0, lse), cu_q, rows)[..., 0]
     sees = _packed((total > 0).float(), cu_q, rows)[..., 0]
-    lse = torch.where(sees > 0, lse, -math.inf).t().contiguous()
+    lse = torch.where(sees > 0, lse, -math.inf)
     return _packed(out, cu_q, rows), lse, (q, k, v, p, out)
 
 
@@ -411,7 +411,7 @@ def _exact_packed(s, lens, new):
     q, k, v = (s[t].detach() for t in ('q', 'k', 'v'))
     group, d = q.shape[1] // k.shape[1], q.shape[2]
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
-    lse = torch.full((q.shape[1], q.shape[0]), -math.inf, dtype=torch.float64, device=q.device)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=q.device)
     dq, dk, dv = (torch.zeros(t.shape, dtype=torch.float64, device=q.device) for t in (q, k, v))
     i0 = j0 = 0
     for n, m in zip(lens, new):
@@ -424,7 +424,7 @@ def _exact_packed(s, lens, new):
             a = qh @ kh.t() / math.sqrt(d)
             if hidden is not None:
                 a[hidden] = -math.inf
-            lse[h, i0:i0 + m] = torch.logsumexp(a, -1)
+            lse[i0:i0 + m, h] = torch.logsumexp(a, -1)
             a = torch.softmax(a, -1)
             out[i0:i0 + m, h] = a @ vh
             if s['kind'] == 'train':
