@@ -566,6 +566,94 @@ int veda_predictor_logits(const float* a, const float* b, int64_t n_heads,
                           const float* log_count, int accumulate, float* out,
                           void* stream);
 
+/*
+ * Attention of packed sequences with grouped heads: sequence b has the queries
+ * [cu_q[b], cu_q[b + 1]) and the keys [cu_k[b], cu_k[b + 1]); query head h
+ * attends with key head h / (n_heads / n_kv_heads). Query i of n_q sees the
+ * keys j <= i + n_k - n_q of n_k when causal, every key otherwise.
+ *   out = softmax(scale q k^T) v,  lse = natural log of the softmax sum
+ * A row that sees no key, and a row of no sequence (before cu_q[0], from
+ * cu_q[n_seq] on), has out = 0 and lse = -inf. A key that a row does not see
+ * does not touch it, whatever it holds.
+ * q, out: bf16 [q_rows, n_heads, D]; k, v: bf16 [k_rows, n_kv_heads, D]; D 64
+ * or 128; strides (stride_s, stride_h, 1), every row 16-byte aligned.
+ * cu_q, cu_k: int32 [n_seq + 1], ascending (offsets outside the rows are
+ * clamped to them). lse: fp32 [q_rows, n_heads] contiguous, or NULL.
+ * scale: positive and finite.
+ */
+int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
+                    const void* k, int64_t k_stride_s, int64_t k_stride_h,
+                    const void* v, int64_t v_stride_s, int64_t v_stride_h,
+                    int64_t q_rows, int64_t k_rows, int64_t n_heads,
+                    int64_t n_kv_heads, int64_t head_dim, const int32_t* cu_q,
+                    const int32_t* cu_k, int64_t n_seq, int causal, float scale,
+                    void* out, int64_t o_stride_s, int64_t o_stride_h,
+                    float* lse, void* stream);
+
+/*
+ * A paged key-value cache: n_pages pages of `page` rows (16, 32, 64, 128 or
+ * 256) of every key head, K and V laid out alike with strides (stride_p,
+ * stride_s, stride_h, 1) of page, row and head in elements, every row 16-byte
+ * aligned. e4m3 0: bf16 rows (k_exp, v_exp unused). e4m3 1: e4m3 codes and an
+ * exponent byte of every row (strides exp_stride_*): the row is codes 2^(byte
+ * - 127), the byte the least that brings the row's largest finite magnitude to
+ * 448 or less; NaN and infinities are held as NaN. Position i of sequence b is
+ * row i % page of page table[b * table_ld + i / page]; a page number outside
+ * [0, n_pages) or a position past `width` pages is no row.
+ *
+ * veda_cache_append writes row cu[b] + i of k and v (bf16 [rows, n_kv_heads,
+ * D]) at position start[b] + i of sequence b; rows of no sequence and
+ * positions of no row are left out. Two rows that meet in one place of the
+ * cache: which of them it then holds is undefined.
+ */
+int veda_cache_append(const void* k, int64_t k_stride_s, int64_t k_stride_h,
+                      const void* v, int64_t v_stride_s, int64_t v_stride_h,
+                      int64_t rows, int64_t n_kv_heads, int64_t head_dim,
+                      const int32_t* cu, const int32_t* start, int64_t n_seq,
+                      void* k_pages, void* v_pages, int64_t stride_p,
+                      int64_t stride_s, int64_t stride_h, int e4m3,
+                      uint8_t* k_exp, uint8_t* v_exp, int64_t exp_stride_p,
+                      int64_t exp_stride_s, int64_t exp_stride_h,
+                      int64_t n_pages, int64_t page, const int32_t* table,
+                      int64_t table_ld, int64_t width, void* stream);
+
+/*
+ * Positions 0, 1, .. of sequence b into rows cu[b], cu[b] + 1, .. cu[b + 1] - 1
+ * of k and v (bf16 [rows, n_kv_heads, D] contiguous); zeros where there is no
+ * row or no sequence.
+ */
+int veda_cache_gather(const void* k_pages, const void* v_pages,
+                      int64_t stride_p, int64_t stride_s, int64_t stride_h,
+                      int e4m3, const uint8_t* k_exp, const uint8_t* v_exp,
+                      int64_t exp_stride_p, int64_t exp_stride_s,
+                      int64_t exp_stride_h, int64_t n_pages, int64_t page,
+                      const int32_t* table, int64_t table_ld, int64_t width,
+                      const int32_t* cu, int64_t n_seq, int64_t rows,
+                      int64_t n_kv_heads, int64_t head_dim, void* k, void* v,
+                      void* stream);
+
+/*
+ * Attention of one new token of every sequence: q [n_seq, n_heads, D] over the
+ * first lengths[b] positions of sequence b (clamped to the table's width;
+ * positions of no row draw no weight). out [n_seq, n_heads, D] bf16, lse fp32
+ * [n_seq, n_heads] contiguous or NULL; out = 0 and lse = -inf without a key.
+ * chunk: keys of a workgroup, a multiple of 32. With n_split = ceil(width *
+ * page / chunk) above 1, workspace holds n_seq * n_heads * n_split * (D + 4)
+ * floats, 16-byte aligned.
+ */
+int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
+                   int64_t n_seq, int64_t n_heads, int64_t n_kv_heads,
+                   int64_t head_dim, const void* k_pages, const void* v_pages,
+                   int64_t stride_p, int64_t stride_s, int64_t stride_h,
+                   int e4m3, const uint8_t* k_exp, const uint8_t* v_exp,
+                   int64_t exp_stride_p, int64_t exp_stride_s,
+                   int64_t exp_stride_h, int64_t n_pages, int64_t page,
+                   const int32_t* table, int64_t table_ld, int64_t width,
+                   const int32_t* lengths, float scale, int64_t chunk,
+                   void* out, int64_t o_stride_s, int64_t o_stride_h,
+                   float* lse, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,14 @@ SIGNATURES: dict[str, list] = {
     'veda_predictor_embed_pair': [_P, _P, _I, _I, _I, _P, _P, _C, _P, _P, _I, _P, _I, _C, _P, _P,
                                   _P],
     'veda_predictor_logits': [_P, _P, _I, _I, _I, _I, _F, _P, _P, _P, _C, _P, _P],
+    'veda_packed_fwd': [_P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _C,
+                        _F, _P, _I, _I, _P, _P],
+    'veda_cache_append': [_P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _C,
+                          _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
+    'veda_cache_gather': [_P, _P, _I, _I, _I, _C, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _I,
+                          _I, _I, _I, _P, _P, _P],
+    'veda_paged_fwd': [_P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I, _I, _C, _P, _P, _I, _I, _I, _I,
+                       _I, _P, _I, _I, _P, _F, _I, _P, _I, _I, _P, _P, _I, _P],
 }
 
 _lock = threading.Lock()

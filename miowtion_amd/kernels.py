@@ -11,6 +11,10 @@ signatures:
   dense_attention                 miowtion/h3/attention.py:28-102
   teacher_heat                    miowtion/kernels/block_heat_triton.py:141-173
 
+and, beside dense_attention, those of packed sequences and the paged cache
+(packed_attention, cache_append_, cache_gather, paged_attention; no reference
+counterpart, `miowtion_amd.packed`).
+
 All run on the GPU through `miowtion_amd.ops`; CPU tensors raise
 NotImplementedError (no fallback, never a silent dense path).
 """
@@ -21,6 +25,8 @@ import torch
 
 from miowtion_amd import ops
 from miowtion_amd import tiling
+from miowtion_amd.packed import (PagedCache, cache_append_, cache_gather, packed_attention,  # noqa: F401
+                                 paged_attention, paged_cache)
 
 SECOND_RAW = 'raw'
 SECOND_CENTRAL = 'central'
@@ -29,8 +35,9 @@ SECOND_CENTRAL = 'central'
 SUPPORTED_ARCH = 'gfx950'
 # head_dim each family of kernels takes: the permutation and pooling kernels
 # are written for 64 and 128 (tile_gather_triton.py:55-66), the attention,
-# heat and compensation kernels for 128 only.
-_HEAD_DIMS = {'gather': (64, 128), 'attention': (128,), 'heat': (128,)}
+# heat and compensation kernels for 128 only, those of packed sequences and the
+# paged cache for both.
+_HEAD_DIMS = {'gather': (64, 128), 'attention': (128,), 'heat': (128,), 'packed': (64, 128)}
 
 
 def _device_arch(device: torch.device) -> str:
@@ -40,7 +47,8 @@ def _device_arch(device: torch.device) -> str:
 def supports(x: torch.Tensor, op: str = 'gather') -> bool:
     """Whether the kernels of `op` ('gather' for gather / pool / scatter,
     'attention' for the sparse and dense forwards, their backward and the
-    compensation, 'heat' for the block heat) can take this tensor: the
+    compensation, 'heat' for the block heat, 'packed' for packed sequences and
+    the paged cache) can take this tensor: the
     library loads, x is a bf16 tensor with a unit last stride and a head_dim
     that family implements, on a gfx950 device. The routing predicate of
     tile_gather_triton.py:55-66: a caller with another path falls through to

@@ -96,7 +96,8 @@ class _Op:
             return self._op(*args, **kwargs)
         out = self._fn(*args)
         for i in self._mutated:
-            torch.autograd.graph.increment_version(args[i])
+            if args[i] is not None:
+                torch.autograd.graph.increment_version(args[i])
         return out
 
     def __getattr__(self, name):

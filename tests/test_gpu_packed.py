@@ -1,0 +1,214 @@
+"""Attention of packed sequences (kernels.packed_attention) against its
+definition in 64 bits: grouped heads, both head dims, causal and not, lengths
+from none to several tiles, rows that see nothing, strides, non-finite values
+where no row looks, and captured graphs."""
+
+import math
+
+import pytest
+import torch
+
+from miowtion_amd import kernels
+from tests import packed_reference as pr
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(lens_q, lens_k, heads, kv, d, seed=0, pad_q=0, pad_k=0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(sum(lens_q) + pad_q, heads, d, generator=g)
+    k = torch.randn(sum(lens_k) + pad_k, kv, d, generator=g)
+    v = torch.randn(sum(lens_k) + pad_k, kv, d, generator=g)
+    return [t.to(torch.bfloat16).cuda() for t in (q, k, v)]
+
+
+CASES = [
+    # lens_q, lens_k (None: lens_q), heads, kv, d, causal
+    ([1], None, 1, 1, 128, True),
+    ([77], None, 40, 8, 128, True),
+    ([1, 2, 3, 64, 65, 127, 128, 129], None, 4, 2, 128, True),
+    ([1, 2, 3, 64, 65, 127, 128, 129], None, 4, 2, 64, True),
+    ([300, 0, 45, 513], None, 6, 2, 128, True),
+    ([300, 0, 45, 513], None, 6, 2, 64, False),
+    ([257, 130], None, 5, 1, 128, False),
+    ([257, 130], None, 7, 7, 64, True),
+    ([1, 17, 128], [700, 17, 1025], 8, 2, 128, True),
+    ([1, 17, 128], [700, 17, 1025], 8, 8, 64, False),
+    ([40, 5, 200], [7, 0, 199], 3, 1, 128, True),    # rows that see nothing
+    ([40, 5, 200], [7, 0, 199], 14, 2, 64, True),
+    ([40, 5, 200], [7, 0, 199], 4, 4, 128, False),
+    ([1100], None, 2, 1, 128, True),
+    ([1500, 9], None, 1, 1, 64, True),
+    ([3] * 150 + [70], None, 4, 2, 64, True),        # more sequences than a wave has lanes
+    ([20], None, 34, 2, 128, True),                   # seventeen heads to a group
+]
+
+
+@pytest.mark.parametrize('case', CASES, ids=lambda c: f'{len(c[0])}x{max(c[0])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}')
+def test_forward(case):
+    lens_q, lens_k, heads, kv, d, causal = case
+    lens_k = lens_k or lens_q
+    print(f'packed forward {case}', flush=True)
+    q, k, v = _inputs(lens_q, lens_k, heads, kv, d)
+    cu_q, cu_k = pr.offsets(lens_q), pr.offsets(lens_k)
+    out, lse = kernels.packed_attention(q, k, v, cu_q, cu_k, causal=causal, return_lse=True)
+    ref = pr.attend(q, k, v, lens_q, lens_k, causal)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+    again = kernels.packed_attention(q, k, v, cu_q, None if lens_k == lens_q else cu_k, causal=causal)
+    assert torch.equal(out, again)
+
+
+def test_scale_and_large_scores():
+    lens = [200, 33]
+    q, k, v = _inputs(lens, lens, 4, 2, 128, seed=3)
+    for scale, grow in ((0.3, 1.0), (1.0, 2.0), (1e-4, 1.0)):
+        out, lse = kernels.packed_attention(q * grow, k, v, pr.offsets(lens), scale=scale, return_lse=True)
+        ref = pr.attend(q * grow, k, v, lens, lens, True, scale)
+        # scores up to 300: a score's error (128 2^-24 of sum |q k| scale, up to
+        # 2,000) is past the bound's share for FP32 work, so it is added here
+        reach = float((q.abs().double().amax() * grow * k.abs().double().amax() * scale) * 128)
+        more = math.expm1(min(reach * 2.0 ** -17, 0.1))
+        ref['out_tol'] = ref['out_tol'] + 2 * more * v.double().abs().amax()
+        pr.check(out, ref, 'out')
+        pr.check(lse, ref, 'lse')
+
+
+def test_rows_of_no_sequence():
+    lens = [50, 200]
+    q, k, v = _inputs(lens, lens, 4, 2, 128, pad_q=150, pad_k=9)
+    k[250:], v[250:] = math.nan, math.inf  # read by nobody
+    q[250:] = math.nan
+    out, lse = kernels.packed_attention(q, k, v, pr.offsets(lens), return_lse=True)
+    ref = pr.attend(q, k, v, lens, lens)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+    assert (out[250:] == 0).all() and (lse[250:] == -math.inf).all()
+    # offsets that do not begin at row 0
+    cu = pr.offsets(lens) + 7
+    out, lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+    assert (out[:7] == 0).all() and (lse[:7] == -math.inf).all()
+    assert (out[257:] == 0).all()
+    ref = pr.attend(q[7:250], k[7:250], v[7:250], [50, 193], [50, 193])
+    pr.check(out[7:57], {n: t[:50] for n, t in ref.items()}, 'out')
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_values_behind_the_mask_do_not_reach_a_row(d):
+    """A later token that is not finite changes no earlier row, and one sequence
+    none of its neighbours."""
+    lens = [90, 200, 70]
+    q, k, v = _inputs(lens, lens, 4, 2, d, seed=5)
+    cu = pr.offsets(lens)
+    clean, clean_lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+    bad_v, bad_k = v.clone(), k.clone()
+    bad_v[90 + 130, 0, 5] = math.nan
+    bad_v[90 + 140, 1] = math.inf
+    bad_k[90 + 150, 0, :3] = math.nan
+    out, lse = kernels.packed_attention(q, bad_k, bad_v, cu, return_lse=True)
+    before = torch.ones(360, dtype=torch.bool)
+    before[90 + 130:290] = False
+    # those rows are formed another way where they shared a tile with the rest
+    ref = pr.attend(q, k, v, lens, lens)
+    ref = {n: t[before] for n, t in ref.items()}
+    pr.check(out[before], ref, 'out')
+    assert torch.equal(lse[before], clean_lse[before])
+    assert torch.isnan(out[90 + 130:290, :2, 5]).all()  # the heads of key head 0 from then on
+    assert torch.isfinite(out[90 + 130:90 + 150, :2, 6]).all()
+    assert (out[90 + 140:290, 2:] == math.inf).all()
+    assert torch.isnan(lse[90 + 150:290, :2]).all()
+    assert torch.equal(out[290:], clean[290:]) and torch.equal(out[:90], clean[:90])
+
+
+def test_strides_and_shared_storage():
+    lens = [130, 61]
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(sum(lens), 8 + 2 + 2, 128, generator=g).to(torch.bfloat16).cuda()
+    q, k, v = qkv.split([8, 2, 2], 1)  # one projection's rows
+    ref = pr.attend(q, k, v, lens, lens)
+    pr.check(kernels.packed_attention(q, k, v, pr.offsets(lens)), ref, 'out')
+    # heads first, and one key head for all by a stride of 0
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)
+    ke, ve = (t[:, :1].expand(-1, 4, -1) for t in (k, v))
+    ref = pr.attend(qt, ke, ve, lens, lens)
+    pr.check(kernels.packed_attention(qt, ke, ve, pr.offsets(lens)), ref, 'out')
+    # every second row
+    q2, k2, v2 = (t[::2] for t in (q, k, v))
+    lens2 = [65, 31]
+    ref = pr.attend(q2, k2, v2, lens2, lens2)
+    pr.check(kernels.packed_attention(q2, k2, v2, pr.offsets(lens2)), ref, 'out')
+
+
+def test_nothing_to_do():
+    q, k, v = _inputs([4], [4], 4, 2, 64)
+    none = torch.zeros(1, dtype=torch.int32, device='cuda')
+    out, lse = kernels.packed_attention(q, k, v, none, return_lse=True)  # no sequence
+    assert (out == 0).all() and (lse == -math.inf).all()
+    assert kernels.packed_attention(q[:0], k, v, torch.zeros(2, dtype=torch.int32, device='cuda')).shape == (0, 4, 64)
+    out = kernels.packed_attention(q, k[:0], v[:0], pr.offsets([4]), torch.zeros(2, dtype=torch.int32, device='cuda'))
+    assert (out == 0).all()
+
+
+def test_offsets_that_make_no_sense_stay_within_the_tensors():
+    q, k, v = _inputs([300], [300], 4, 2, 128)
+    guard = torch.full((64, 4, 128), 7.0, dtype=torch.bfloat16, device='cuda')
+    for cu in ([0, 500], [-5, 10, 100000], [200, 100, 300], [300, 0], [5, 5, 5]):
+        print(f'offsets {cu}', flush=True)
+        out = kernels.packed_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device='cuda'))
+        assert out.shape == q.shape
+    assert (guard == 7.0).all()
+    out = kernels.packed_attention(q, k, v, torch.tensor([0, 500], dtype=torch.int32, device='cuda'))
+    pr.check(out, pr.attend(q, k, v, [300], [300]), 'out')
+
+
+def test_graph_serves_new_lengths():
+    q, k, v = _inputs([300], [300], 4, 2, 128)
+    cu = pr.offsets([100, 200])
+    kernels.packed_attention(q, k, v, cu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+    for lens in ([100, 200], [1, 299], [300, 0], [17, 100]):
+        cu.copy_(pr.offsets(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        pr.check(out, pr.attend(q, k, v, lens, lens), 'out')
+
+
+def test_side_stream_and_inference_mode():
+    lens = [200]
+    q, k, v = _inputs(lens, lens, 4, 2, 128)
+    cu = pr.offsets(lens)
+    want = kernels.packed_attention(q, k, v, cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.inference_mode():
+        out = kernels.packed_attention(q, k, v, cu)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want)
+
+
+def test_refusals():
+    q, k, v = _inputs([16], [16], 4, 2, 128)
+    cu = pr.offsets([16])
+    f = kernels.packed_attention
+    for bad, match in [
+            (lambda: f(q.float(), k, v, cu), 'bfloat16'),
+            (lambda: f(q[0], k, v, cu), 'rows, heads'),
+            (lambda: f(q, k[..., :64], v[..., :64], cu), 'head_dim'),
+            (lambda: f(q[..., :96], k[..., :96], v[..., :96], cu), 'head_dim'),
+            (lambda: f(q[:, :3], k, v, cu), 'multiple'),
+            (lambda: f(q, k, v[:8], cu), 'equal shapes'),
+            (lambda: f(q, k, v, cu.long()), 'int32'),
+            (lambda: f(q, k, v, cu, cu[:1]), 'int32'),
+            (lambda: f(q, k, v, cu, scale=0.0), 'scale'),
+            (lambda: f(q, k, v, cu, scale=-1.0), 'scale'),
+            (lambda: f(q, k, v, cu, scale=math.nan), 'scale'),
+            (lambda: f(q.new_empty(16 * 4 * 128 + 8)[4:-4].view(16, 4, 128), k, v, cu), '16-byte')]:
+        with pytest.raises(ValueError, match=match):
+            bad()
+    with pytest.raises((ValueError, NotImplementedError)):
+        f(q, k, v, cu.cpu())
