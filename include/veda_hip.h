@@ -591,6 +591,26 @@ int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                     float* lse, void* stream);
 
 /*
+ * Gradients of veda_packed_fwd: with P = exp(S - lse), D = rowsum(dout out) -
+ * dlse and dS = P (dout v^T - D), dq = scale dS k, dk = scale dS^T q and dv =
+ * P^T dout, dk and dv summed over the query heads of a key head. Rows of no
+ * sequence and rows that see (or are seen by) nothing get zeros. Every row is
+ * written by one workgroup: the same bits on every call.
+ * out, lse: what the forward gave (lse [q_rows, n_heads] contiguous). dlse: fp32
+ * as lse, or NULL. dq [q_rows, n_heads, D], dk, dv [k_rows, n_kv_heads, D]:
+ * bf16 contiguous. workspace: 16-byte aligned, 1,024 bytes for each of n_kv_heads *
+ * (q_rows * (n_heads / n_kv_heads) / 128 + n_seq + 2).
+ */
+int veda_packed_bwd(
+    const void* q, int64_t q_stride_s, int64_t q_stride_h, const void* k, int64_t k_stride_s,
+    int64_t k_stride_h, const void* v, int64_t v_stride_s, int64_t v_stride_h, const void* out,
+    int64_t o_stride_s, int64_t o_stride_h, const void* dout, int64_t do_stride_s,
+    int64_t do_stride_h, const float* lse, const float* dlse, int64_t q_rows, int64_t k_rows,
+    int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const int32_t* cu_q,
+    const int32_t* cu_k, int64_t n_seq, int causal, float scale, void* dq, void* dk, void* dv,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * A paged key-value cache: n_pages pages of `page` rows (16, 32, 64, 128 or
  * 256) of every key head, K and V laid out alike with strides (stride_p,
  * stride_s, stride_h, 1) of page, row and head in elements, every row 16-byte

@@ -11,7 +11,7 @@ import contextlib
 import torch
 
 from miowtion_amd import _native
-from miowtion_amd.ops import _check_rows, _custom_op, _p, _stream
+from miowtion_amd.ops import TILE, _check_rows, _custom_op, _p, _stream
 
 HEAD_DIMS = (64, 128)
 PAGES = (16, 32, 64, 128, 256)
@@ -83,6 +83,41 @@ def packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Te
 def _(q, k, v, cu_q, cu_k, causal, scale, return_lse):
     out = q.new_empty(q.shape)
     return [out, q.new_empty(q.shape[:2], dtype=torch.float32)] if return_lse else [out]
+
+
+@_custom_op('veda::packed_bwd', mutates_args=())
+def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+               dout: torch.Tensor, lse: torch.Tensor, dlse: torch.Tensor | None,
+               cu_q: torch.Tensor, cu_k: torch.Tensor, causal: bool,
+               scale: float) -> list[torch.Tensor]:
+    """[dq, dk, dv] of packed_fwd, from its out and lse."""
+    _check_packed(q, k, v, cu_q, cu_k, scale)
+    for name, t in (('out', out), ('dout', dout)):
+        _check_rows(name, t)
+        _check_aligned(name, t)
+        if t.shape != q.shape or t.device != q.device:
+            raise ValueError(f'{name} {tuple(t.shape)} must be as q {tuple(q.shape)}')
+    for name, t in (('lse', lse), ('dlse', dlse)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:2]
+                              or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f'{name} must be contiguous fp32 {list(q.shape[:2])}')
+    rows, heads, d = q.shape
+    kv, n_seq = k.shape[1], cu_q.shape[0] - 1
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    work = torch.empty(kv * (rows * (heads // kv) // TILE + n_seq + 2) * 256, dtype=torch.float32,
+                       device=q.device)
+    with _on(q):
+        _native.call('veda_packed_bwd', q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k),
+                     v.data_ptr(), *_strides(v), out.data_ptr(), *_strides(out), dout.data_ptr(),
+                     *_strides(dout), lse.data_ptr(), _p(dlse), rows, k.shape[0], heads, kv, d,
+                     cu_q.data_ptr(), cu_k.data_ptr(), n_seq, int(causal), scale, dq.data_ptr(),
+                     dk.data_ptr(), dv.data_ptr(), work.data_ptr(), 4 * work.numel(), _stream(q))
+    return [dq, dk, dv]
+
+
+@packed_bwd.register_fake
+def _(q, k, v, out, dout, lse, dlse, cu_q, cu_k, causal, scale):
+    return [t.new_empty(t.shape) for t in (q, k, v)]
 
 
 # --------------------------------------------------------------------------

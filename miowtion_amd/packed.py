@@ -55,6 +55,28 @@ def _scale(scale: float | None, head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
 
 
+class _PackedAttention(torch.autograd.Function):
+    """packed_attention with gradients of q, k and v, through out and the LSE."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
+        out, lse = ops_packed.packed_fwd(q, k, v, cu_q, cu_k, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.causal, ctx.scale = causal, scale
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        dout = torch.zeros_like(out) if dout is None else dout.contiguous()
+        dq, dk, dv = ops_packed.packed_bwd(q, k, v, out, dout, lse,
+                                           None if dlse is None else dlse.contiguous(), cu_q, cu_k,
+                                           ctx.causal, ctx.scale)
+        return dq, dk, dv, None, None, None, None
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: torch.Tensor | None = None, causal: bool = True,
                      scale: float | None = None, return_lse: bool = False):
@@ -76,10 +98,16 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     Returns:
         out [Tq, H, D] bf16, or (out, lse). Rows that see no key, and rows of no
         sequence, have out 0 and lse -inf. A key that a row does not see does not
-        touch its out, whatever it holds.
+        touch its out, whatever it holds. Differentiable in q, k and v (and
+        through the LSE) where they require grad, once; the gradients are the same
+        bits on every call, and values that are not finite stay within the
+        gradients of their sequence.
     """
     scale = _scale(scale, q.shape[-1])
     cu_k = cu_q if cu_k is None else cu_k
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, causal, scale)
+        return (out, lse) if return_lse else out
     res = ops_packed.packed_fwd(q, k, v, cu_q, cu_k, causal, scale, return_lse)
     return (res[0], res[1]) if return_lse else res[0]
 
