@@ -11,6 +11,15 @@
 //       keys in steps of 64. It forms D from its rows of O and dO and leaves
 //       [LSE log2 e | -D] of every 64 rows as a record for the other kernel.
 //       Transposed products (S^T = K Q^T): a lane owns a query row.
+//       The dS of a row sum to dLSE. With D from the bf16 O they do not: D is
+//       off by 2^-9 of |dO| |O| and every dS by 2^-9 of itself, and what their
+//       sum is off by meets the row's mean key P K, which is no small vector
+//       where keys have a direction in common. So the kernel adds up dS (exact,
+//       which mends D for the records) and its rounded values, forms P K with
+//       the products' A operand that dS K has read already, and takes the
+//       rounded sum's excess times P K off dQ. Distance of dQ from 64 bits at
+//       8,192 tokens x 28 heads: 1.1e-2 -> 2.1e-3 (bf16's own rounding is
+//       1.7e-3), of dK 5e-3 -> 2.4e-3; the whole step 7 % longer.
 //   packed_dkv_kernel  128 keys of one key head, the packed rows that see them
 //       in steps of 64. Plain products (S = Q K^T): a lane owns a key.
 // In both, P or dS goes from the accumulators straight into the B operand of
@@ -59,6 +68,22 @@ __device__ __forceinline__ int lane_anew() {
   return ln;
 }
 
+// Offsets of a lane's reads in a tile of rows permuted by swz_both. Row reads:
+// row lane % 32, chunk 2 s + lane / 32 is row_offset xor 32 s. Transposed reads:
+// column block t is tr_offset xor 64 t, the next eight rows xor 8 kPitch + 32.
+template <int D>
+__device__ __forceinline__ uint32_t row_offset(int lane) {
+  const int li = lane & 31;
+  return (uint32_t)(li * Tile<D>::kPitch + (((lane >> 5) ^ swz_both<D>(li)) << 4));
+}
+
+// acc + the two bf16 of a word.
+__device__ __forceinline__ float add_pair(uint32_t pair, float acc) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair),
+                                         __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
+}
+
 // 32 rows of a wave as whole rows from its accumulators (acc[t][e] = row
 // lane % 32, column 32 t + 8 (e / 4) + 4 (lane / 32) + e % 4), by way of `stage`;
 // row(i) is where row i goes, or NULL.
@@ -90,7 +115,11 @@ template <int D>
 __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   using T = Tile<D>;
   constexpr int kSlot = 2 * T::kBytes;  // K and V of a step
+  // of head_dim 128 half of the wave's Q fragments stay in LDS: with the two
+  // sums of products a row has, all of them would not fit the registers
+  constexpr int kQReg = D == 128 ? T::kK / 2 : T::kK;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[2][kSlot];
+  __shared__ __attribute__((aligned(1024))) uint8_t qbox[D == 128 ? 4 * 4096 : 16];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
@@ -110,13 +139,16 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   const int64_t token = sp.q0 + r / group;
   const int64_t qhead = (int64_t)head * group + r % group;
   const int64_t n_heads = (int64_t)p.pk.n_kv * group;
-  bf16x8 qf[T::kK], dof[T::kK];
+  bf16x8 qf[kQReg], dof[T::kK];
+  lds_u8* const qmine = (lds_u8*)qbox + wave * 4096;
   float dot = 0.f;
   const bf16x8 zero = as_bf16x8(u32x4{0, 0, 0, 0});
 #pragma unroll
   for (int s = 0; s < T::kK; ++s) {
     const int d = 16 * s + 8 * hi;
-    qf[s] = real ? as_bf16x8(ld16(p.q + token * p.qs + qhead * p.qh + d)) : zero;
+    const bf16x8 qx = real ? as_bf16x8(ld16(p.q + token * p.qs + qhead * p.qh + d)) : zero;
+    if (s < kQReg) qf[s] = qx;
+    else *reinterpret_cast<lds_u32x4*>(qmine + ((s - kQReg) * 64 + lane) * 16) = __builtin_bit_cast(u32x4, qx);
     dof[s] = real ? as_bf16x8(ld16(p.dout + token * p.dos + qhead * p.doh + d)) : zero;
     const u32x4 a = __builtin_bit_cast(u32x4, dof[s]);
     const u32x4 b = real ? ld16(p.o + token * p.os + qhead * p.oh + d) : u32x4{0, 0, 0, 0};
@@ -134,15 +166,11 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
     lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
     nd = (p.dlse != nullptr ? p.dlse[token * n_heads + qhead] : 0.f) - dot;
   }
-  if (hi == 0) {
-    float* rec = p.rec + (((int64_t)head * p.q_slots + slot) * 2 + (wave >> 1)) * kRecFloats;
-    rec[32 * (wave & 1) + li] = lse2;
-    rec[64 + 32 * (wave & 1) + li] = nd;
-  }
 
   const uint16_t* kbase = p.k + (int64_t)sp.k0 * p.ks + head * p.kh;
   const uint16_t* vbase = p.v + (int64_t)sp.k0 * p.vs + head * p.vh;
   auto load_step = [&](int u, lds_u8* dst) {
+    const int lane = lane_anew();
     const char* kb = reinterpret_cast<const char*>(kbase + (int64_t)u * 64 * p.ks);
     const char* vb = reinterpret_cast<const char*>(vbase + (int64_t)u * 64 * p.vs);
 #pragma unroll
@@ -155,13 +183,10 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
             dst + T::kBytes + seg * 1024);
     }
   };
-  // row reads: chunk 2 s + hi is base xor 32 s; transposed: column block t is
-  // base xor 64 t, the next eight rows base xor (8 rows, swizzle bit 1)
-  const uint32_t ra = (uint32_t)(li * T::kPitch + ((hi ^ swz_both<D>(li)) << 4));
-  const uint32_t ta = tr_offset<D>(lane, 0, 0, swz_both<D>);
-  f32x16 acc[T::kT];
+  f32x16 acc[T::kT], mean[T::kT];  // dS K, P K
 #pragma unroll
-  for (int t = 0; t < T::kT; ++t) acc[t] = zero16();
+  for (int t = 0; t < T::kT; ++t) acc[t] = mean[t] = zero16();
+  float sum = 0.f, sum_r = 0.f;  // of dS, and of dS as rounded
   const float c = p.scale_log2;
 
   lds_u8* const s0 = (lds_u8*)ring[0];
@@ -172,40 +197,78 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (u + 1 < n_steps) load_step(u + 1, s0 + ((u + 1) & 1) * kSlot);
-#pragma unroll
+#pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
+      const int ln = lane_anew();
+      const uint32_t ra = row_offset<D>(ln), ta = tr_offset<D>(ln, 0, 0, swz_both<D>);
       const lds_u8* ks = cur + sub * 32 * T::kPitch;
       const lds_u8* vs = ks + T::kBytes;
       f32x16 st = zero16(), dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] = nd;
+      bf16x8 ka[T::kK], va[T::kK];
+      ka[0] = lds_frag(ks + ra);
+      va[0] = lds_frag(vs + ra);
 #pragma unroll
       for (int s = 0; s < T::kK; ++s) {
-        st = mfma32(lds_frag(ks + (ra ^ (32 * s))), qf[s], st);
-        dp = mfma32(lds_frag(vs + (ra ^ (32 * s))), dof[s], dp);
-      }
-      float ds[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -lse2)) * dp[e];
-      if (u >= n_plain) {
-        const int lim = limit - 64 * u - 32 * sub - 4 * hi;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (8 * (e >> 2) + (e & 3) >= lim) ds[e] = 0.f;
-      }
-      u32x4 pb[2];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pb[j >> 2][j & 3] = pack_bf16x2(ds[2 * j], ds[2 * j + 1]);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int t = 0; t < T::kT; ++t) {
-          const lds_u8* a = ks + kk * 16 * T::kPitch;
-          const uint32_t at = ta ^ (64 * t);
-          acc[t] = mfma32(join_tr(a + at, a + (at ^ (8 * T::kPitch + 32))), as_bf16x8(pb[kk]), acc[t]);
+        if (s + 1 < T::kK) {
+          ka[s + 1] = lds_frag(ks + (ra ^ (32 * (s + 1))));
+          va[s + 1] = lds_frag(vs + (ra ^ (32 * (s + 1))));
         }
+        st = mfma32(ka[s], s < kQReg ? qf[s % kQReg] : lds_frag(qmine + ((s - kQReg) * 64 + ln) * 16), st);
+        dp = mfma32(va[s], dof[s], dp);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const int lim = u >= n_plain ? limit - 64 * u - 32 * sub - 4 * hi : 32;
+      u32x4 pb[2], db[2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float pr[2], ds[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int e = 2 * j + m;
+          const bool see = 8 * (e >> 2) + (e & 3) < lim;
+          pr[m] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -lse2));
+          ds[m] = see ? pr[m] * dp[e] : 0.f;
+          pr[m] = see ? pr[m] : 0.f;
+        }
+        pb[j >> 2][j & 3] = pack_bf16x2(pr[0], pr[1]);
+        const uint32_t y = pack_bf16x2(ds[0], ds[1]);
+        db[j >> 2][j & 3] = y;
+        sum += ds[0] + ds[1];
+        sum_r = add_pair(y, sum_r);
+      }
+      auto tr = [&](int i) {  // keys 16 (i / kT), column block i % kT
+        const lds_u8* a = ks + (i / T::kT) * 16 * T::kPitch;
+        const uint32_t at = ta ^ (64 * (i % T::kT));
+        return join_tr(a + at, a + (at ^ (8 * T::kPitch + 32)));
+      };
+      bf16x8 kt[2 * T::kT];
+      kt[0] = tr(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2 * T::kT; ++i) {
+        if (i + 1 < 2 * T::kT) kt[i + 1] = tr(i + 1);
+        acc[i % T::kT] = mfma32(kt[i], as_bf16x8(db[i / T::kT]), acc[i % T::kT]);
+        mean[i % T::kT] = mfma32(kt[i], as_bf16x8(pb[i / T::kT]), mean[i % T::kT]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
+  // dS of a row sums to dLSE: what its rounded values sum to beside that has
+  // gone to the row's mean key, and -D is off by what the exact ones do
+  sum = half_swap_sum(sum);
+  sum_r = half_swap_sum(sum_r);
+  const float dl = real && p.dlse != nullptr && lse2 != INFINITY ? p.dlse[token * n_heads + qhead] : 0.f;
+  if (hi == 0) {
+    float* rec = p.rec + (((int64_t)head * p.q_slots + slot) * 2 + (wave >> 1)) * kRecFloats;
+    rec[32 * (wave & 1) + li] = lse2;
+    rec[64 + 32 * (wave & 1) + li] = nd - (sum - dl);
+  }
+#pragma unroll
+  for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(dl - sum_r, mean[t][e], acc[t][e]);
   __syncthreads();  // every wave is done with the ring
   uint16_t* const mine = p.dq + (token * n_heads + qhead) * D;
   const uint64_t bits = reinterpret_cast<uintptr_t>(mine);
@@ -291,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   // rows 32 b .. + 31 of step u; MASK: some of them do not see all of the keys
   auto compute = [&](auto mask, int u, int b, const lds_u8* cur) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask)::value;
-    const int ln = lane_anew(), li = ln & 31, hi = ln >> 5;
-    const uint32_t ra = (uint32_t)(li * T::kPitch + ((hi ^ swz_both<D>(li)) << 4));
+    const int ln = lane_anew(), hi = ln >> 5;
+    const uint32_t ra = row_offset<D>(ln);
     const uint32_t ta = tr_offset<D>(ln, 0, 0, swz_both<D>);
     const lds_u8* qs = cur + b * 32 * T::kPitch;
     const lds_u8* ds = qs + T::kBytes;
