@@ -598,8 +598,10 @@ int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
  * written by one workgroup: the same bits on every call.
  * out, lse: what the forward gave (lse [q_rows, n_heads] contiguous). dlse: fp32
  * as lse, or NULL. dq [q_rows, n_heads, D], dk, dv [k_rows, n_kv_heads, D]:
- * bf16 contiguous. workspace: 16-byte aligned, 1,024 bytes for each of n_kv_heads *
- * (q_rows * (n_heads / n_kv_heads) / 128 + n_seq + 2).
+ * bf16 contiguous. n_split (1 .. 64): workgroups that share the query rows of a key
+ * tile. workspace: 16-byte aligned, 1,024 bytes for each of n_kv_heads * (q_rows *
+ * (n_heads / n_kv_heads) / 128 + n_seq + 2), and with n_split > 1 another 8 * n_split
+ * bytes for each value of dk.
  */
 int veda_packed_bwd(
     const void* q, int64_t q_stride_s, int64_t q_stride_h, const void* k, int64_t k_stride_s,
@@ -607,7 +609,7 @@ int veda_packed_bwd(
     int64_t o_stride_s, int64_t o_stride_h, const void* dout, int64_t do_stride_s,
     int64_t do_stride_h, const float* lse, const float* dlse, int64_t q_rows, int64_t k_rows,
     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const int32_t* cu_q,
-    const int32_t* cu_k, int64_t n_seq, int causal, float scale, void* dq, void* dk, void* dv,
+    const int32_t* cu_k, int64_t n_seq, int causal, float scale, int64_t n_split, void* dq, void* dk, void* dv,
     void* workspace, int64_t workspace_bytes, void* stream);
 
 /*

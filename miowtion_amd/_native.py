@@ -74,7 +74,7 @@ SIGNATURES: dict[str, list] = {
     'veda_packed_fwd': [_P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _C,
                         _F, _P, _I, _I, _P, _P],
     'veda_packed_bwd': [_P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I,
-                        _I, _I, _I, _P, _P, _I, _C, _F, _P, _P, _P, _P, _I, _P],
+                        _I, _I, _I, _P, _P, _I, _C, _F, _I, _P, _P, _P, _P, _I, _P],
     'veda_cache_append': [_P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _C,
                           _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
     'veda_cache_gather': [_P, _P, _I, _I, _I, _C, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _I,

@@ -9,6 +9,8 @@
 // computed transposed (S^T = K Q^T, 32x32x16 products), so a lane owns one
 // query row, its softmax needs one exchange between the wave's halves, and P^T
 // goes from the accumulators into the B operand of O^T += V^T P^T.
+#include <type_traits>
+
 #include "packed_common.h"
 
 namespace veda {
@@ -65,6 +67,163 @@ __device__ __noinline__ void redo_row(const uint16_t* q, const uint16_t* k, cons
   for (int m = 0; m < D / 64; ++m) out[lane + 64 * m] = (uint16_t)f32_to_bf16(acc[m] * inv);
 }
 
+// ---------------------------------------------------------------------------
+// A stage works on three consecutive 32-key sub-blocks at once: the score
+// products of sub-block n + 1 (QK: K rows at `kb` into sn), the softmax of n (SM:
+// scores sp into the packed probabilities pn) and the P V products of n - 1 (PV: V
+// rows at `vb`, probabilities pp), written out in turn with scheduling fences, so
+// that a wave's vector and matrix work run at once. A stage is one basic block:
+// a branch inside it would make the compiler move the softmax out of it or keep
+// O twice, so O's rescale waits for the next stage's start (alpha).
+//
+// The reference of a row is the maximum of its first step; later probabilities
+// are taken against it as it stands, with no maximum taken, unless a lane's 16
+// sum to kLazyLimit or more, or are not finite, or a row has no reference yet:
+// then the sub-block raises the references that a score passes by 2^8 and takes
+// its probabilities again.
+
+constexpr float kLazyLimit = 256.f;
+constexpr float kRescaleSlack = 8.f;  // log2 units
+
+template <int D>
+struct Wave {
+  bf16x8 qf[Tile<D>::kK];
+  f32x16 o[Tile<D>::kT];
+  float m_run, l_run, mu;  // mu: m_run, or 0 where there is none
+  float alpha;             // what O is still to be scaled by
+  bool have_ref;           // every row of the wave has a reference
+  float first_sum;         // of a step's first sub-block, until the second's joins it
+};
+
+enum { kNoSm = 0, kSmFirst = 1, kSmSecond = 2 };
+
+template <int D>
+__device__ __forceinline__ void raise_reference(const f32x16& s, float c, u32x4 (&pk)[2], Wave<D>& w) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
+  top = half_swap_max(top) * c;
+  const float m_new = top > w.m_run + kRescaleSlack ? top : w.m_run;
+  const float mu = m_new == -INFINITY ? 0.f : m_new;
+  w.alpha = __builtin_amdgcn_exp2f(w.m_run - mu);
+  w.m_run = m_new;
+  w.mu = mu;
+  float l4[4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = __builtin_amdgcn_exp2f(fmaf(s[2 * j], c, -mu));
+    const float b = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], c, -mu));
+    l4[j >> 1] = (j & 1) ? l4[j >> 1] + (a + b) : a + b;
+    pk[j >> 2][j & 3] = pack_bf16x2(a, b);
+  }
+  w.l_run = fmaf(w.l_run, w.alpha, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+  w.have_ref = __ballot(m_new != -INFINITY) == ~0ull;
+}
+
+template <int D>
+__device__ __forceinline__ void first_reference(const f32x16& sa, const f32x16& sb, float c, Wave<D>& w) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(sa[e], sb[e]));
+  w.m_run = half_swap_max(top) * c;
+  w.mu = w.m_run == -INFINITY ? 0.f : w.m_run;
+  w.have_ref = __ballot(w.m_run != -INFINITY) == ~0ull;
+}
+
+// Scores of keys that a row does not see; lim: the row's keys less the
+// sub-block's first one.
+__device__ __forceinline__ void mask_scores(f32x16& s, int lim, int hi) {
+  const int l = lim - 4 * hi;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (8 * (e >> 2) + (e & 3) >= l) s[e] = -INFINITY;
+}
+
+template <int D>
+struct Frags {
+  uint32_t k[Tile<D>::kK];  // K row li, chunk 2 s + hi
+  uint32_t v[Tile<D>::kT];  // transposed reads of V
+};
+
+// First fragments of the stage that follows on the same slots, read in the place
+// of a stage's last reads, so that its products do not begin with a wait.
+template <int D>
+struct Next {
+  bf16x8 k[Tile<D>::kK / 2];
+  bf16x8 v;
+};
+enum { kNoNext = 0, kReadNext = 1, kTakeNext = 2 };
+
+template <int D>
+__device__ __forceinline__ bf16x8 vt_frag(const lds_u8* vb, const Frags<D>& f, int i) {
+  const lds_u8* a = vb + (i / Tile<D>::kT) * 16 * Tile<D>::kPitch + f.v[i % Tile<D>::kT];
+  return join_tr(a, a + 8 * Tile<D>::kPitch);
+}
+
+template <int D, bool QK, int SM, bool PV, int NEXT = kNoNext, typename Hook>
+__device__ __forceinline__ void stage(const lds_u8* kb, const lds_u8* vb, const Frags<D>& f, float c,
+                                      f32x16& sn, const f32x16& sp, u32x4 (&pn)[2],
+                                      const u32x4 (&pp)[2], Wave<D>& w, Hook hook,
+                                      Next<D>* next = nullptr) {
+  using T = Tile<D>;
+  constexpr int kAhead = T::kK / 2;          // K fragments ahead of their products
+  constexpr int kEvery = 8 / T::kK;          // pieces for a product of each kind
+  constexpr int kSub = 32 * T::kPitch;       // bytes of 32 rows
+  if (PV && __any(w.alpha != 1.f)) {
+#pragma unroll
+    for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w.o[t][e] *= w.alpha;
+  }
+  bf16x8 kf[T::kK], va[T::kK];
+  if (QK) {
+    sn = zero16();
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) kf[k] = NEXT == kTakeNext ? next->k[k] : lds_frag(kb + f.k[k]);
+  }
+  if (PV) va[0] = NEXT == kTakeNext ? next->v : vt_frag<D>(vb, f, 0);
+  float l4[4];
+  const float mu = w.mu;
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    hook(j);
+    const int i = j / kEvery;
+    if (QK && j % kEvery == 0) {
+      if (i + kAhead < T::kK) kf[i + kAhead] = lds_frag(kb + f.k[i + kAhead]);
+      else if (NEXT == kReadNext) next->k[i - kAhead] = lds_frag(kb + kSub + f.k[i - kAhead]);
+      sn = mfma32(kf[i], w.qf[i], sn);
+    }
+    if (SM != kNoSm) {
+      const float a = __builtin_amdgcn_exp2f(fmaf(sp[2 * j], c, -mu));
+      const float b = __builtin_amdgcn_exp2f(fmaf(sp[2 * j + 1], c, -mu));
+      l4[j >> 1] = (j & 1) ? l4[j >> 1] + (a + b) : a + b;
+      uint32_t pk = pack_bf16x2(a, b);
+      asm volatile("" : "+v"(pk));  // kept here, not sunk to its use a stage later
+      pn[j >> 2][j & 3] = pk;
+    }
+    if (PV && j % kEvery == kEvery - 1) {
+      if (i + 1 < T::kK) va[i + 1] = vt_frag<D>(vb, f, i + 1);
+      else if (NEXT == kReadNext) next->v = vt_frag<D>(vb + kSub, f, 0);
+      w.o[i % T::kT] = mfma32(va[i], as_bf16x8(pp[i / T::kT]), w.o[i % T::kT]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  w.alpha = 1.f;
+  if (SM != kNoSm) {
+    const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+    if (__builtin_expect(!(w.have_ref && __ballot(sum < kLazyLimit) == ~0ull), 0)) {
+      if (SM == kSmSecond) w.l_run += w.first_sum;
+      w.first_sum = 0.f;
+      raise_reference<D>(sp, c, pn, w);
+    } else if (SM == kSmFirst) {
+      w.first_sum = sum;
+    } else {
+      w.l_run += w.first_sum + sum;
+    }
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   using T = Tile<D>;
@@ -89,90 +248,118 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int64_t token = sp.q0 + r / p.pk.group;
   const int64_t qhead = (int64_t)head * p.pk.group + r % p.pk.group;
   const uint16_t* qptr = p.q + token * p.qs + qhead * p.qh;
-  bf16x8 qf[T::kK];
+  Wave<D> w;
 #pragma unroll
   for (int s = 0; s < T::kK; ++s)
-    qf[s] = real ? as_bf16x8(ld16(qptr + 16 * s + 8 * hi)) : as_bf16x8(u32x4{0, 0, 0, 0});
+    w.qf[s] = real ? as_bf16x8(ld16(qptr + 16 * s + 8 * hi)) : as_bf16x8(u32x4{0, 0, 0, 0});
 
   const uint16_t* kbase = p.k + (int64_t)sp.k0 * p.ks + head * p.kh;
   const uint16_t* vbase = p.v + (int64_t)sp.k0 * p.vs + head * p.vh;
-  // K and V of step u; rows past the sequence's last key read that key again
-  auto load_step = [&](int u, lds_u8* dst) {
-    const char* kb = reinterpret_cast<const char*>(kbase + (int64_t)u * 64 * p.ks);
-    const char* vb = reinterpret_cast<const char*>(vbase + (int64_t)u * 64 * p.vs);
+  // This wave's loads of K or V of step u (past the last step that one again):
+  // segment s is 1 KB, rows kSegRows (kSegs wave + s) on; rows past the
+  // sequence's last key read that key again.
+  struct Src {
+    const char* base;
+    uint32_t off[T::kSegs];
+  };
+  auto src_of = [&](const uint16_t* x, int64_t stride, int u, bool is_v, bool clamp) {
+    u = clamp ? min(u, n_steps - 1) : u;
+    Src r;
+    r.base = reinterpret_cast<const char*>(x + (int64_t)u * 64 * stride);
 #pragma unroll
     for (int s = 0; s < T::kSegs; ++s) {
-      const int seg = T::kSegs * wave + s;
-      const int row = seg * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
-      const int src = min(row, sp.nk - 1 - 64 * u);
-      dma16(kb, (uint32_t)src * (uint32_t)(2 * p.ks) + ((pos ^ swz_row<D>(row)) << 4), dst + seg * 1024);
-      dma16(vb, (uint32_t)src * (uint32_t)(2 * p.vs) + ((pos ^ swz_tr<D>(row)) << 4),
-            dst + T::kBytes + seg * 1024);
+      const int row = (T::kSegs * wave + s) * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
+      const uint32_t src = (uint32_t)(clamp ? min(row, sp.nk - 1 - 64 * u) : row);
+      r.off[s] = src * (uint32_t)(2 * stride) +
+                 ((pos ^ (is_v ? swz_tr<D>(row) : swz_row<D>(row))) << 4);
     }
+    return r;
   };
-  uint32_t kro[T::kK], vro[T::kT];
+  Frags<D> f;
 #pragma unroll
   for (int s = 0; s < T::kK; ++s)
-    kro[s] = (uint32_t)(li * T::kPitch + (((2 * s + hi) ^ swz_row<D>(li)) << 4));
+    f.k[s] = (uint32_t)(li * T::kPitch + (((2 * s + hi) ^ swz_row<D>(li)) << 4));
 #pragma unroll
-  for (int t = 0; t < T::kT; ++t) vro[t] = T::kBytes + tr_offset<D>(lane, t, 0, swz_tr<D>);
-
-  f32x16 o[T::kT];
+  for (int t = 0; t < T::kT; ++t) f.v[t] = T::kBytes + tr_offset<D>(lane, t, 0, swz_tr<D>);
 #pragma unroll
-  for (int t = 0; t < T::kT; ++t) o[t] = zero16();
-  float m_run = -INFINITY, l_run = 0.f;
+  for (int t = 0; t < T::kT; ++t) w.o[t] = zero16();
+  w.m_run = -INFINITY;
+  w.l_run = w.mu = w.first_sum = 0.f;
+  w.alpha = 1.f;
+  w.have_ref = false;
   const float c = p.scale_log2;
 
+  // The walk. K and V of step u have their halves of slot u % 2, and V runs one
+  // step behind K: iteration u multiplies K of step u + 1 and V of step u, and
+  // loads K of step u + 2 (over K of step u) and V of step u + 1, so a load has
+  // an iteration to arrive.
+  constexpr int kSub = 32 * T::kPitch;
   lds_u8* const s0 = (lds_u8*)ring[0];
-  if (n_steps > 0) load_step(0, s0);
-  for (int u = 0; u < n_steps; ++u) {
-    const lds_u8* cur = s0 + (u & 1) * kSlot;
+  const uint32_t lds0 =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(s0 + T::kSegs * 1024 * wave));
+  auto issue = [&](const Src& x, int s, uint32_t to) { dma16_m0(x.base, x.off[s], to + s * 1024); };
+  auto sync = [&]() {
     VEDA_WAIT_VM(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (u + 1 < n_steps) load_step(u + 1, s0 + ((u + 1) & 1) * kSlot);
+  };
+  f32x16 sa, sb;
+  u32x4 pa[2], pb[2];
+  auto iter = [&](auto masked, int u, uint32_t cur, uint32_t nxt) __attribute__((always_inline)) {
+    // MASKED: step u + 1 holds keys that some row does not see, or step u + 2 may
+    // be past the last
+    constexpr bool MASKED = decltype(masked)::value;
+    const Src ks = src_of(kbase, p.ks, u + 2, false, MASKED);
+    const Src vs = src_of(vbase, p.vs, u + 1, true, MASKED);
+    sync();
+    auto hook = [&](int j) {
+      if (j < T::kSegs) issue(ks, j, lds0 + cur);
+      else if (j < 2 * T::kSegs) issue(vs, j - T::kSegs, lds0 + nxt + T::kBytes);
+    };
+    Next<D> next;
+    stage<D, true, kSmSecond, true, kReadNext>(s0 + nxt, s0 + cur, f, c, sa, sb, pb, pa, w, hook, &next);
+    if (MASKED) mask_scores(sa, limit - 64 * (u + 1), hi);
+    stage<D, true, kSmFirst, true, kTakeNext>(s0 + nxt + kSub, s0 + cur + kSub, f, c, sb, sa, pa, pb, w,
+                                              NoHook{}, &next);
+    if (MASKED) mask_scores(sb, limit - 64 * (u + 1) - 32, hi);
+  };
+  if (n_steps > 0) {
+    const Src k0 = src_of(kbase, p.ks, 0, false, true), k1 = src_of(kbase, p.ks, 1, false, true);
+    const Src v0 = src_of(vbase, p.vs, 0, true, true);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      f32x16 s = zero16();
+    for (int s = 0; s < T::kSegs; ++s) issue(k0, s, lds0);
 #pragma unroll
-      for (int i = 0; i < T::kK; ++i)
-        s = mfma32(lds_frag(cur + sub * 32 * T::kPitch + kro[i]), qf[i], s);
-      if (u >= n_plain) {
-        const int lim = limit - 64 * u - 32 * sub - 4 * hi;
+    for (int s = 0; s < T::kSegs; ++s) issue(k1, s, lds0 + kSlot);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (8 * (e >> 2) + (e & 3) >= lim) s[e] = -INFINITY;
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
-      const float m_new = fmaxf(m_run, half_swap_max(top) * c);
-      const float mu = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
-      m_run = m_new;
-      float sum = 0.f;
-      u32x4 pb[2];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = __builtin_amdgcn_exp2f(fmaf(s[2 * j], c, -mu));
-        const float b = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], c, -mu));
-        sum += a + b;
-        pb[j >> 2][j & 3] = pack_bf16x2(a, b);
-      }
-      l_run = fmaf(l_run, alpha, sum);
-#pragma unroll
-      for (int t = 0; t < T::kT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int t = 0; t < T::kT; ++t) {
-          const lds_u8* a = cur + (sub * 32 + kk * 16) * T::kPitch + vro[t];
-          o[t] = mfma32(join_tr(a, a + 8 * T::kPitch), as_bf16x8(pb[kk]), o[t]);
-        }
+    for (int s = 0; s < T::kSegs; ++s) issue(v0, s, lds0 + T::kBytes);
+    VEDA_WAIT_VM(2 * T::kSegs);  // K of step 0; K of step 1 and V of step 0 may be in flight
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    stage<D, true, kNoSm, false>(s0, s0, f, c, sa, sb, pb, pa, w, NoHook{});
+    stage<D, true, kNoSm, false>(s0 + kSub, s0, f, c, sb, sa, pa, pb, w, NoHook{});
+    if (n_plain == 0) {
+      mask_scores(sa, limit, hi);
+      mask_scores(sb, limit - 32, hi);
     }
+    first_reference<D>(sa, sb, c, w);
+    stage<D, false, kSmFirst, false>(s0, s0, f, c, sb, sa, pa, pb, w, NoHook{});
+    int u = 0;
+    for (; u + 3 < n_plain; u += 2) {
+      iter(std::false_type{}, u, 0, kSlot);
+      iter(std::false_type{}, u + 1, kSlot, 0);
+    }
+#pragma unroll 1
+    for (; u + 1 < n_steps; ++u) {
+      const uint32_t at = (u & 1) * kSlot;
+      iter(std::true_type{}, u, at, kSlot - at);
+    }
+    const lds_u8* const cur = s0 + ((n_steps - 1) & 1) * kSlot;
+    sync();
+    stage<D, false, kSmSecond, true>(s0, cur, f, c, sb, sb, pb, pa, w, NoHook{});
+    stage<D, false, kNoSm, true>(s0, cur + kSub, f, c, sa, sb, pa, pb, w, NoHook{});
   }
+  const float m_run = w.m_run, l_run = w.l_run;
+  f32x16(&o)[T::kT] = w.o;
 
   // O leaves as whole rows, by way of the wave's part of the ring
   const float l = half_swap_sum(l_run);

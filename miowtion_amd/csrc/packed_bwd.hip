@@ -56,8 +56,9 @@ struct BwdArgs {
   uint16_t* dq;       // [q_rows, H, D]
   uint16_t* dk;       // [k_rows, n_kv, D]
   uint16_t* dv;
+  float* part;        // [dv | dk][n_split][k_rows, n_kv, D] sums, with n_split > 1
   float scale, scale_log2;
-  int32_t q_slots, k_slots;
+  int32_t q_slots, k_slots, n_split;
 };
 
 // The lane's index, formed anew at each call, so that what is derived from it
@@ -291,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
-  const int slot = (int)(blockIdx.x / p.pk.n_kv);  // causal: the first keys have the most rows
+  const int item = (int)(blockIdx.x / p.pk.n_kv);
+  const int slot = item / p.n_split, split = item % p.n_split;  // causal: the first keys have the most rows
   const Span sp = span_of_slot(p.pk, true, slot, lane);
   const int j0 = sp.tile * kRows;
   if (j0 >= sp.nk) return;
@@ -301,7 +303,10 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
     const int64_t i = (int64_t)j - (sp.nk - sp.nq);
     return p.pk.causal ? (int)min(max(i * group, (int64_t)0), (int64_t)rows) : 0;
   };
-  const int u0 = first(j0) >> 6, u1 = (rows + 63) >> 6;
+  const int first_step = first(j0) >> 6, end_step = (rows + 63) >> 6;  // the steps that see the tile, and this split's
+  const int n_all = max(end_step - first_step, 0);
+  const int u0 = first_step + (int)((int64_t)n_all * split / p.n_split);
+  const int u1 = first_step + (int)((int64_t)n_all * (split + 1) / p.n_split);
   const int w0 = j0 + 32 * wave;                       // this wave's keys
   const int key = min(w0 + li, sp.nk - 1);
   const int mine = first(key);
@@ -460,10 +465,42 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   const int64_t base = (int64_t)(sp.k0 + w0) * ld + (int64_t)head * D;
   lds_u8* const stage = s0 + wave * 32 * T::kPitch;
   const int ln = lane_anew();
+  if (p.n_split > 1) {
+    // sums in 32 bits, joined and rounded by packed_join_kernel
+    if (w0 + (ln & 31) >= sp.nk) return;
+    float* to = p.part + split * ((int64_t)p.pk.k_rows * ld) + base + (ln & 31) * ld + 4 * (ln >> 5);
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      const f32x16(&a)[T::kT] = pass == 0 ? acc_v : acc_k;
+#pragma unroll
+      for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(to + 32 * t + 8 * g) =
+              f32x4{a[t][4 * g], a[t][4 * g + 1], a[t][4 * g + 2], a[t][4 * g + 3]};
+      to += (int64_t)p.n_split * p.pk.k_rows * ld;
+    }
+    return;
+  }
   store_rows<D>(acc_v, 1.f, stage, ln,
                 [&](int rr) { return w0 + rr < sp.nk ? p.dv + base + rr * ld : nullptr; });
   store_rows<D>(acc_k, p.scale, stage, ln,
                 [&](int rr) { return w0 + rr < sp.nk ? p.dk + base + rr * ld : nullptr; });
+}
+
+// The splits' sums of dV and dK joined: a thread four values, in the order of
+// the splits.
+__global__ void __launch_bounds__(256) packed_join_kernel(const float* part, int64_t n, int n_split,
+                                                          float scale, uint16_t* dv, uint16_t* dk) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const bool is_k = blockIdx.y != 0;
+  const float* x = part + (is_k ? n_split * n : 0) + i;
+  f32x4 s = *reinterpret_cast<const f32x4*>(x);
+  for (int k = 1; k < n_split; ++k) s += *reinterpret_cast<const f32x4*>(x + k * n);
+  const float m = is_k ? scale : 1.f;
+  *reinterpret_cast<u32x2*>((is_k ? dk : dv) + i) =
+      u32x2{pack_bf16x2(s[0] * m, s[1] * m), pack_bf16x2(s[2] * m, s[3] * m)};
 }
 
 }  // namespace
@@ -477,7 +514,7 @@ extern "C" int veda_packed_bwd(
     int64_t o_stride_s, int64_t o_stride_h, const void* dout, int64_t do_stride_s,
     int64_t do_stride_h, const float* lse, const float* dlse, int64_t q_rows, int64_t k_rows,
     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const int32_t* cu_q,
-    const int32_t* cu_k, int64_t n_seq, int causal, float scale, void* dq, void* dk, void* dv,
+    const int32_t* cu_k, int64_t n_seq, int causal, float scale, int64_t n_split, void* dq, void* dk, void* dv,
     void* workspace, int64_t workspace_bytes, void* stream) {
   VEDA_REQUIRE(head_dim == 64 || head_dim == 128, "packed_bwd: head_dim must be 64 or 128, got %lld",
                (long long)head_dim);
@@ -506,7 +543,11 @@ extern "C" int veda_packed_bwd(
   const int64_t q_slots = slots_of(q_rows, p.pk.group, n_seq), k_slots = slots_of(k_rows, 1, n_seq);
   VEDA_REQUIRE(q_slots * n_kv_heads < (1ll << 31) && k_slots * n_kv_heads < (1ll << 31),
                "packed_bwd: too many tiles");
-  const int64_t need = q_slots * n_kv_heads * 2 * kRecBytes;
+  VEDA_REQUIRE(n_split >= 1 && n_split <= 64 && k_slots * n_kv_heads * n_split < (1ll << 31),
+               "packed_bwd: n_split %lld outside [1, 64], or too many tiles", (long long)n_split);
+  const int64_t n_out = k_rows * n_kv_heads * head_dim;
+  const int64_t rec_bytes = q_slots * n_kv_heads * 2 * kRecBytes;
+  const int64_t need = rec_bytes + (n_split > 1 ? 2 * n_split * n_out * 4 : 0);
   VEDA_REQUIRE(workspace != nullptr && rows16(workspace, 0, 0) && workspace_bytes >= need,
                "packed_bwd: workspace needs %lld bytes (16-byte aligned), got %lld", (long long)need,
                (long long)workspace_bytes);
@@ -523,6 +564,8 @@ extern "C" int veda_packed_bwd(
   p.lse = lse;
   p.dlse = dlse;
   p.rec = static_cast<float*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + rec_bytes);
+  p.n_split = (int32_t)n_split;
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
@@ -531,7 +574,7 @@ extern "C" int veda_packed_bwd(
   p.q_slots = (int32_t)q_slots;
   p.k_slots = (int32_t)k_slots;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned q_grid = (unsigned)(q_slots * n_kv_heads), k_grid = (unsigned)(k_slots * n_kv_heads);
+  const unsigned q_grid = (unsigned)(q_slots * n_kv_heads), k_grid = (unsigned)(k_slots * n_kv_heads * n_split);
   if (q_rows > 0) {
     if (head_dim == 128) packed_dq_kernel<128><<<q_grid, kThreads, 0, s>>>(p);
     else packed_dq_kernel<64><<<q_grid, kThreads, 0, s>>>(p);
@@ -540,6 +583,11 @@ extern "C" int veda_packed_bwd(
   if (k_rows > 0) {
     if (head_dim == 128) packed_dkv_kernel<128><<<k_grid, kThreads, 0, s>>>(p);
     else packed_dkv_kernel<64><<<k_grid, kThreads, 0, s>>>(p);
+    if (n_split > 1) {
+      if (int rc = check_launch("veda_packed_bwd (dk, dv)")) return rc;
+      packed_join_kernel<<<dim3((unsigned)((n_out / 4 + 255) / 256), 2), 256, 0, s>>>(
+          p.part, n_out, p.n_split, scale, p.dv, p.dk);
+    }
   }
   return check_launch("veda_packed_bwd (dk, dv)");
 }
