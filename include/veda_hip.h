@@ -579,7 +579,9 @@ int veda_predictor_logits(const float* a, const float* b, int64_t n_heads,
  * or 128; strides (stride_s, stride_h, 1), every row 16-byte aligned.
  * cu_q, cu_k: int32 [n_seq + 1], ascending (offsets outside the rows are
  * clamped to them). lse: fp32 [q_rows, n_heads] contiguous, or NULL.
- * scale: positive and finite.
+ * scale: positive and finite. n_split (1 .. 64): workgroups that share the keys
+ * of 128 rows; above 1, workspace holds n_split * q_rows * n_heads * (D + 2)
+ * floats, 16-byte aligned.
  */
 int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                     const void* k, int64_t k_stride_s, int64_t k_stride_h,
@@ -587,8 +589,9 @@ int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                     int64_t q_rows, int64_t k_rows, int64_t n_heads,
                     int64_t n_kv_heads, int64_t head_dim, const int32_t* cu_q,
                     const int32_t* cu_k, int64_t n_seq, int causal, float scale,
-                    void* out, int64_t o_stride_s, int64_t o_stride_h,
-                    float* lse, void* stream);
+                    int64_t n_split, void* out, int64_t o_stride_s,
+                    int64_t o_stride_h, float* lse, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 /*
  * Gradients of veda_packed_fwd: with P = exp(S - lse), D = rowsum(dout out) -
@@ -659,7 +662,7 @@ int veda_cache_gather(const void* k_pages, const void* v_pages,
  * first lengths[b] positions of sequence b (clamped to the table's width;
  * positions of no row draw no weight). out [n_seq, n_heads, D] bf16, lse fp32
  * [n_seq, n_heads] contiguous or NULL; out = 0 and lse = -inf without a key.
- * chunk: keys of a workgroup, a multiple of 32. With n_split = ceil(width *
+ * chunk: keys of a workgroup, a multiple of 32 and 1 to 64 whole pages. With n_split = ceil(width *
  * page / chunk) above 1, workspace holds n_seq * n_heads * n_split * (D + 4)
  * floats, 16-byte aligned.
  */

@@ -72,7 +72,7 @@ SIGNATURES: dict[str, list] = {
                                   _P],
     'veda_predictor_logits': [_P, _P, _I, _I, _I, _I, _F, _P, _P, _P, _C, _P, _P],
     'veda_packed_fwd': [_P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _C,
-                        _F, _P, _I, _I, _P, _P],
+                        _F, _I, _P, _I, _I, _P, _P, _I, _P],
     'veda_packed_bwd': [_P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _I,
                         _I, _I, _I, _P, _P, _I, _C, _F, _I, _P, _P, _P, _P, _I, _P],
     'veda_cache_append': [_P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _C,

@@ -19,6 +19,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 struct FwdArgs {
   Packing pk;
   const uint16_t* q;
@@ -28,18 +31,21 @@ struct FwdArgs {
   uint16_t* out;
   int64_t os, oh;
   float* lse;  // [q_rows, H] or NULL
+  float* part;  // n_split > 1: [n_split][q_rows, H][D] sums, then [n_split][q_rows, H]
+                // pairs of reference (log2) and sum of weights
   float scale_log2;
-  int32_t n_slots;
+  int32_t n_slots, n_split;
 };
 
 // A row whose O came out with an infinity or a NaN, again, key by key: a key
 // that the row does not see, or whose probability is zero, adds nothing
 // whatever its V holds (a product with a zero probability makes a NaN of it).
-// All lanes of the wave work on the row; lane l has head-dims l and l + 64.
+// All lanes of the wave work on the row; lane l has head-dims l and l + 64. To
+// out as bf16, or, where part is given, there in 32 bits.
 template <int D>
 __device__ __noinline__ void redo_row(const uint16_t* q, const uint16_t* k, const uint16_t* v,
                                       int64_t ks, int64_t vs, int limit, float c, float mu, float inv,
-                                      uint16_t* out, int lane) {
+                                      uint16_t* out, float* part, int lane) {
   float acc[D / 64] = {};
   for (int j0 = 0; j0 < limit; j0 += 64) {
     const int j = j0 + lane;
@@ -64,7 +70,10 @@ __device__ __noinline__ void redo_row(const uint16_t* q, const uint16_t* k, cons
     }
   }
 #pragma unroll
-  for (int m = 0; m < D / 64; ++m) out[lane + 64 * m] = (uint16_t)f32_to_bf16(acc[m] * inv);
+  for (int m = 0; m < D / 64; ++m) {
+    if (part != nullptr) part[lane + 64 * m] = acc[m];
+    else out[lane + 64 * m] = (uint16_t)f32_to_bf16(acc[m] * inv);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -233,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
-  const int slot = p.n_slots - 1 - (int)(blockIdx.x / p.pk.n_kv);
+  const int item = (int)(blockIdx.x / p.pk.n_kv);
+  const int slot = p.n_slots - 1 - item / p.n_split, split = item % p.n_split;
   const Span sp = span_of_slot(p.pk, false, slot, lane);
   const int rows = sp.nq * p.pk.group;
   const int r0 = sp.tile * kRows;
@@ -242,9 +252,14 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int r = r0 + 32 * wave + li;
   const bool real = r < rows;
   const int last = visible_keys(p.pk, sp, min(r0 + kRows, rows) - 1);
-  const int limit = real ? visible_keys(p.pk, sp, r) : last;
-  const int n_steps = (last + 63) >> 6;
-  const int n_plain = visible_keys(p.pk, sp, r0) >> 6;  // steps that every row sees whole
+  // this split's steps of 64 keys; from here on keys count from its first
+  const int all_steps = (last + 63) >> 6;
+  const int from = (int)((int64_t)all_steps * split / p.n_split);
+  const int n_steps = (int)((int64_t)all_steps * (split + 1) / p.n_split) - from;
+  const int end = 64 * n_steps;
+  const int limit = min(max((real ? visible_keys(p.pk, sp, r) : last) - 64 * from, 0), end);
+  const int n_plain = min(max(visible_keys(p.pk, sp, r0) - 64 * from, 0), end) >> 6;  // seen whole by every row
+  const int nk = sp.nk - 64 * from;
   const int64_t token = sp.q0 + r / p.pk.group;
   const int64_t qhead = (int64_t)head * p.pk.group + r % p.pk.group;
   const uint16_t* qptr = p.q + token * p.qs + qhead * p.qh;
@@ -253,8 +268,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   for (int s = 0; s < T::kK; ++s)
     w.qf[s] = real ? as_bf16x8(ld16(qptr + 16 * s + 8 * hi)) : as_bf16x8(u32x4{0, 0, 0, 0});
 
-  const uint16_t* kbase = p.k + (int64_t)sp.k0 * p.ks + head * p.kh;
-  const uint16_t* vbase = p.v + (int64_t)sp.k0 * p.vs + head * p.vh;
+  const uint16_t* kbase = p.k + (int64_t)(sp.k0 + 64 * from) * p.ks + head * p.kh;
+  const uint16_t* vbase = p.v + (int64_t)(sp.k0 + 64 * from) * p.vs + head * p.vh;
   // This wave's loads of K or V of step u (past the last step that one again):
   // segment s is 1 KB, rows kSegRows (kSegs wave + s) on; rows past the
   // sequence's last key read that key again.
@@ -269,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
 #pragma unroll
     for (int s = 0; s < T::kSegs; ++s) {
       const int row = (T::kSegs * wave + s) * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
-      const uint32_t src = (uint32_t)(clamp ? min(row, sp.nk - 1 - 64 * u) : row);
+      const uint32_t src = (uint32_t)(clamp ? min(row, nk - 1 - 64 * u) : row);
       r.off[s] = src * (uint32_t)(2 * stride) +
                  ((pos ^ (is_v ? swz_tr<D>(row) : swz_row<D>(row))) << 4);
     }
@@ -364,9 +379,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   // O leaves as whole rows, by way of the wave's part of the ring
   const float l = half_swap_sum(l_run);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (p.lse != nullptr && hi == 0 && real)
-    p.lse[token * ((int64_t)p.pk.n_kv * p.pk.group) + qhead] =
-        l == 0.f ? -INFINITY : (m_run + __log2f(l)) * kLn2;
+  const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;
+  if (p.lse != nullptr && hi == 0 && real && p.n_split == 1)
+    p.lse[token * n_heads + qhead] = l == 0.f ? -INFINITY : (m_run + __log2f(l)) * kLn2;
   bool bad = false;
 #pragma unroll
   for (int t = 0; t < T::kT; ++t)
@@ -374,8 +389,37 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
     for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[t][e]) < INFINITY);
   const uint64_t bad_lanes = __ballot(bad);
   uint32_t bad_rows = (uint32_t)bad_lanes | (uint32_t)(bad_lanes >> 32);
+  auto redo = [&](uint32_t which) {
+    while (which != 0) {
+      const int rr = __builtin_ctz(which);
+      which &= which - 1;
+      const int row = r0 + 32 * wave + rr;
+      if (row >= rows) continue;
+      const int64_t tok = sp.q0 + row / p.pk.group, hd = (int64_t)head * p.pk.group + row % p.pk.group;
+      const float m = __shfl(m_run, rr);
+      redo_row<D>(p.q + tok * p.qs + hd * p.qh, kbase, vbase, p.ks, p.vs, __shfl(limit, rr), c,
+                  m == -INFINITY ? 0.f : m, __shfl(inv, rr), p.out + tok * p.os + hd * p.oh,
+                  p.n_split > 1 ? p.part + (split * all_rows + tok * n_heads + hd) * D : nullptr, lane);
+    }
+  };
+  if (p.n_split > 1) {
+    if (real) {
+      const int64_t at = split * all_rows + token * n_heads + qhead;
+      if (hi == 0)
+        *reinterpret_cast<f32x2*>(p.part + p.n_split * all_rows * D + 2 * at) = f32x2{m_run, l};
+      if (!((bad_rows >> li) & 1)) {
+#pragma unroll
+        for (int t = 0; t < T::kT; ++t)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(p.part + at * D + 32 * t + 8 * g + 4 * hi) =
+                f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+      }
+    }
+    redo(bad_rows);
+    return;
+  }
   __syncthreads();  // every wave is done with the ring
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   lds_u8* const stage = s0 + wave * 32 * T::kPitch;
 #pragma unroll
   for (int t = 0; t < T::kT; ++t)
@@ -399,16 +443,35 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
       *reinterpret_cast<u32x4*>(
           reinterpret_cast<uint16_t*>((uintptr_t)(((uint64_t)up << 32) | lo)) + 8 * pos) = x;
   }
-  while (bad_rows != 0) {
-    const int rr = __builtin_ctz(bad_rows);
-    bad_rows &= bad_rows - 1;
-    const int row = r0 + 32 * wave + rr;
-    if (row >= rows) continue;
-    const int64_t tok = sp.q0 + row / p.pk.group, hd = (int64_t)head * p.pk.group + row % p.pk.group;
-    const float m = __shfl(m_run, rr);
-    redo_row<D>(p.q + tok * p.qs + hd * p.qh, kbase, vbase, p.ks, p.vs, __shfl(limit, rr), c,
-                m == -INFINITY ? 0.f : m, __shfl(inv, rr), p.out + tok * p.os + hd * p.oh, lane);
+  redo(bad_rows);
+}
+
+// The splits of a row joined: D / 4 threads a row, four head-dims each.
+template <int D>
+__global__ void __launch_bounds__(256) packed_merge_kernel(FwdArgs p) {
+  const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (D / 4);
+  const int d = 4 * (int)(i % (D / 4));
+  if (row >= all_rows) return;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(p.part + p.n_split * all_rows * D) + row;
+  float m = -INFINITY;
+  for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, ml[s * all_rows][0]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.n_split; ++s) {
+    const f32x2 x = ml[s * all_rows];
+    const float w = __builtin_amdgcn_exp2f(x[0] - mu);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part + (s * all_rows + row) * D + d);
+    l = fmaf(w, x[1], l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, y[e], o[e]);
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.out + (row / n_heads) * p.os + (row % n_heads) * p.oh + d) =
+      u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+  if (d == 0 && p.lse != nullptr) p.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 }  // namespace
@@ -421,8 +484,9 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
                                int64_t v_stride_s, int64_t v_stride_h, int64_t q_rows,
                                int64_t k_rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                                const int32_t* cu_q, const int32_t* cu_k, int64_t n_seq, int causal,
-                               float scale, void* out, int64_t o_stride_s, int64_t o_stride_h,
-                               float* lse, void* stream) {
+                               float scale, int64_t n_split, void* out, int64_t o_stride_s,
+                               int64_t o_stride_h, float* lse, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   VEDA_REQUIRE(head_dim == 64 || head_dim == 128, "packed_fwd: head_dim must be 64 or 128, got %lld",
                (long long)head_dim);
   VEDA_REQUIRE(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0,
@@ -453,13 +517,28 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
   p.lse = lse;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int64_t slots = slots_of(q_rows, p.pk.group, n_seq);
-  VEDA_REQUIRE(slots * n_kv_heads < (1ll << 31), "packed_fwd: too many tiles");
+  VEDA_REQUIRE(n_split >= 1 && n_split <= 64 && slots * n_kv_heads * n_split < (1ll << 31),
+               "packed_fwd: n_split %lld outside [1, 64], or too many tiles", (long long)n_split);
+  const int64_t need = n_split == 1 ? 0 : n_split * q_rows * n_heads * (head_dim + 2) * 4;
+  VEDA_REQUIRE(need == 0 || (workspace != nullptr && rows16(workspace, 0, 0) && workspace_bytes >= need),
+               "packed_fwd: workspace needs %lld bytes (16-byte aligned), got %lld", (long long)need,
+               (long long)workspace_bytes);
+  p.part = static_cast<float*>(workspace);
+  p.n_split = (int32_t)n_split;
   p.n_slots = (int32_t)slots;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned grid = (unsigned)(slots * n_kv_heads);
+  const unsigned grid = (unsigned)(slots * n_kv_heads * n_split);
   if (head_dim == 128)
     packed_fwd_kernel<128><<<grid, kThreads, 0, s>>>(p);
   else
     packed_fwd_kernel<64><<<grid, kThreads, 0, s>>>(p);
+  if (n_split > 1) {
+    if (int rc = check_launch("packed_fwd")) return rc;
+    const unsigned join = (unsigned)((q_rows * n_heads * (head_dim / 4) + 255) / 256);
+    if (head_dim == 128)
+      packed_merge_kernel<128><<<join, 256, 0, s>>>(p);
+    else
+      packed_merge_kernel<64><<<join, 256, 0, s>>>(p);
+  }
   return check_launch("packed_fwd");
 }

@@ -228,6 +228,11 @@ __global__ void __launch_bounds__(256) gather_cache_kernel(GatherArgs p) {
 // B operand of O^T += V^T P^T when k index e of lane group g stands for key
 // 16 (e / 4) + 4 g + e % 4. K goes from memory straight into the A operand; V
 // passes through the wave's own LDS, to be read transposed.
+//
+// Bound by the cache's bytes: a tile's K is asked for once the last tile's
+// scores are formed, its V once the last one's is in LDS, so a wave has a tile in
+// flight at all times in the registers of one. The chunk's page numbers are in
+// one register from the start (lane i: page i of the chunk).
 
 struct TokenArgs {
   const uint16_t* q;
@@ -240,7 +245,7 @@ struct TokenArgs {
   uint16_t* out;
   int64_t os, oh;
   float* lse;   // [B, H] or NULL
-  float* part;  // [B, H, n_split, D + 2]: O, then the reference (log2) and the sum
+  float* part;  // [B, H, n_split, D + 4]: O, then the reference (log2) and the sum
 };
 
 template <int D>
@@ -257,17 +262,25 @@ __device__ __forceinline__ float over_groups(float v) {
   return MAX ? half_swap_max(v) : half_swap_sum(v);
 }
 
+__device__ __forceinline__ int length_of(const TokenArgs& p, int b) {
+  const int capacity = (int)min((int64_t)p.tab.width << p.tab.shift, (int64_t)0x7fffffff);
+  return min(max(p.lengths[b], 0), capacity);
+}
+
 template <int D, bool F8>
-__global__ void __launch_bounds__(256) token_kernel(TokenArgs p) {
+__global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   constexpr int kPitch = 2 * D;               // a V row in LDS, bf16
   constexpr int kTileBytes = 32 * kPitch;
   constexpr int kPer = F8 ? 16 : 8;           // elements of a 16-byte load
+  constexpr int kBytes = F8 ? 1 : 2;
   constexpr int kKLoads = D / (4 * kPer);     // of a lane, for a K row
   constexpr int kSteps = D / 32;              // k-steps of a score
   constexpr int kLanes = D / kPer;            // lanes of a V row
-  constexpr int kVRows = 64 / kLanes;         // V rows of a load
+  constexpr int kVRows = 64 / kLanes;         // V rows of a load (at most 16: one block of keys)
   constexpr int kVLoads = 32 / kVRows;
   constexpr int kDB = D / 16;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
   __shared__ __attribute__((aligned(1024))) uint8_t vt[4 * kTileBytes];
   __shared__ float red_m[4][16], red_l[4][16];
   const int tid = threadIdx.x;
@@ -278,13 +291,20 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs p) {
   const int head = blockIdx.x % p.n_kv;
   const int g0 = 16 * blockIdx.z;             // first query head of the group here
   const int split = blockIdx.x / p.n_kv;
-  const int capacity = (int)min((int64_t)p.tab.width << p.tab.shift, (int64_t)0x7fffffff);
-  const int len = min(max(p.lengths[b], 0), capacity);
   const int begin = split * p.chunk;
+  const int len = length_of(p, b);
   if (begin >= len && split > 0) return;      // the join does not read it
   const int end = min(begin + p.chunk, len);
   const int nq = min(p.group - g0, 16);
 
+  // the chunk's pages, -1 where there is none (64 at most)
+  const int first_page = begin >> p.tab.shift;
+  int pages = -1;
+  if (begin < len) {
+    const int i = min(first_page + lane, (len - 1) >> p.tab.shift);
+    pages = p.tab.t[b * p.tab.ld + i];
+    pages = pages >= 0 && pages < p.tab.pages ? pages : -1;
+  }
   // Q: query head n, in the order of the K loads' elements
   bf16x8 qf[kSteps];
   const uint16_t* qrow = p.q + b * p.qs + ((int64_t)head * p.group + g0 + min(n, nq - 1)) * p.qh;
@@ -292,78 +312,62 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs p) {
   for (int s = 0; s < kSteps; ++s)
     qf[s] = as_bf16x8(ld16(qrow + (F8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g)));
 
-  struct Loaded {
-    u32x4 k[2][kKLoads], v[kVLoads];
-    uint32_t ke[2], ve[kVLoads];
-    int live;  // bit i: block i of 16 keys has a page
-  };
   const int mask = (1 << p.tab.shift) - 1;
-  const int last_page = max(len - 1, 0) >> p.tab.shift;
-  const int32_t* trow = p.tab.t + b * p.tab.ld;
   const int vr = lane / kLanes, vd = kPer * (lane % kLanes);
-  constexpr int kBytes = F8 ? 1 : 2;
-  auto load = [&](int j0, Loaded& x) __attribute__((always_inline)) {
-    // the tile's two pages (the same one but for 16-row pages): wave-uniform
-    int pg[2];
-    x.live = 0;
+  // a head's first row of a page, wave-uniform; a lane's row and columns from
+  // there are 32-bit offsets (the launcher checks)
+  const uint8_t* const kx = p.kp.x + head * p.kp.sh * kBytes;
+  const uint8_t* const vx = p.vp.x + head * p.vp.sh * kBytes;
+  const uint8_t* const kex = F8 ? p.kp.e + head * p.kp.eh : nullptr;
+  const uint8_t* const vex = F8 ? p.vp.e + head * p.vp.eh : nullptr;
+  const uint32_t row_bytes = (uint32_t)(p.kp.ss * kBytes), row_exps = (uint32_t)p.kp.es;
+  auto page_at = [&](int j) { return __builtin_amdgcn_readlane(pages, (j >> p.tab.shift) - first_page); };
+  // Block i of 16 keys of the tile at j0 lies in one page. Past the sequence's
+  // end its rows are the rest of the last page, which no row's score or
+  // probability takes in.
+  u32x4 kreg[2][kKLoads], vreg[kVLoads];
+  uint32_t ke[2], ve[kVLoads];
+  auto load_k = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      pg[i] = trow[min((j0 + 16 * i) >> p.tab.shift, last_page)];
-      const bool ok = pg[i] >= 0 && pg[i] < p.tab.pages;
-      x.live |= ok ? 1 << i : 0;
-      pg[i] = ok ? pg[i] : 0;
-    }
+      const int64_t pg = max(page_at(j0 + 16 * i), 0);
+      const uint32_t at = (uint32_t)((j0 + 16 * i + n) & mask);
+      const uint8_t* page = kx + pg * p.kp.sp * kBytes;
+      const uint32_t off = at * row_bytes + 16 * g;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int64_t at = (j0 + 16 * i + n) & mask;
-      const uint8_t* row = p.kp.x + (pg[i] * p.kp.sp + at * p.kp.ss + head * p.kp.sh) * kBytes;
-#pragma unroll
-      for (int s = 0; s < kKLoads; ++s)
-        x.k[i][s] = *reinterpret_cast<const u32x4*>(row + 64 * s + 16 * g);
-      if (F8) x.ke[i] = p.kp.e[pg[i] * p.kp.ep + at * p.kp.es + head * p.kp.eh];
+      for (int s = 0; s < kKLoads; ++s) kreg[i][s] = *reinterpret_cast<const u32x4*>(page + (off + 64 * s));
+      if (F8) ke[i] = (kex + pg * p.kp.ep)[at * row_exps];
     }
+  };
+  auto load_v = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < kVLoads; ++u) {
-      const int row = kVRows * u + vr;
-      const int64_t page = kVRows * u < 16 ? pg[0] : pg[1];  // kVRows <= 16: a load is in one block
-      const int64_t at = (j0 + row) & mask;
-      x.v[u] = *reinterpret_cast<const u32x4*>(
-          p.vp.x + (page * p.vp.sp + at * p.vp.ss + head * p.vp.sh + vd) * kBytes);
-      if (F8) x.ve[u] = p.vp.e[page * p.vp.ep + at * p.vp.es + head * p.vp.eh];
+      const int64_t pg = max(page_at(j0 + (kVRows * u < 16 ? 0 : 16)), 0);
+      const uint32_t at = (uint32_t)((j0 + kVRows * u + vr) & mask);
+      vreg[u] = *reinterpret_cast<const u32x4*>(vx + pg * p.vp.sp * kBytes + (at * row_bytes + vd * kBytes));
+      if (F8) ve[u] = (vex + pg * p.vp.ep)[at * row_exps];
     }
   };
 
   lds_u8* const mine = (lds_u8*)vt + wave * kTileBytes;
-  uint32_t tr[kDB];
-#pragma unroll
-  for (int db = 0; db < kDB; ++db) {
-    const int r = 4 * g + (n >> 2);
-    tr[db] = (uint32_t)(r * kPitch + (((2 * db + ((n >> 1) & 1)) ^ swz_v<D>(r)) << 4) + 8 * (n & 1));
-  }
+  // transposed reads: rows 4 g + n / 4 (and 16 on), column block db at xor 32 db
+  const int tr_row = 4 * g + (n >> 2);
+  const uint32_t tr = (uint32_t)(tr_row * kPitch + ((((n >> 1) & 1) ^ swz_v<D>(tr_row)) << 4) + 8 * (n & 1));
   f32x4 o[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.f;
   const float c = p.scale_log2;
 
-  auto tile = [&](int j0, const Loaded& x) __attribute__((always_inline)) {
-    // V into LDS, zero where there is no key
-#pragma unroll
-    for (int u = 0; u < kVLoads; ++u) {
-      const int row = kVRows * u + vr;
-      const bool ok = j0 + row < end && ((x.live >> (kVRows * u < 16 ? 0 : 1)) & 1);
-      lds_u8* const to = mine + row * kPitch;
-      const int ch = vd / 8, sw = swz_v<D>(row);
-      typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-      if (F8) {
-        u32x4 a, d;
-        decode16(x.v[u], scale_of(x.ve[u]), a, d);
-        *reinterpret_cast<lds_u32x4*>(to + ((ch ^ sw) << 4)) = ok ? a : u32x4{0, 0, 0, 0};
-        *reinterpret_cast<lds_u32x4*>(to + (((ch + 1) ^ sw) << 4)) = ok ? d : u32x4{0, 0, 0, 0};
-      } else {
-        *reinterpret_cast<lds_u32x4*>(to + ((ch ^ sw) << 4)) = ok ? x.v[u] : u32x4{0, 0, 0, 0};
-      }
-    }
+  int j = begin + 32 * wave;
+  if (p.tab.pages == 0) j = end;
+  if (j < end) {
+    load_k(j);
+    load_v(j);
+  }
+  for (; j < end; j += 128) {
+    const bool more = j + 128 < end;
+    const int live[2] = {page_at(j) >= 0 ? end - j : 0, page_at(j + 16) >= 0 ? end - j - 16 : 0};
     f32x4 s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -371,17 +375,20 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs p) {
       u32x4 a[kSteps];
 #pragma unroll
       for (int t = 0; t < kKLoads; ++t) {
-        if (F8) decode16(x.k[i][t], scale_of(x.ke[i]), a[(2 * t) % kSteps], a[(2 * t + 1) % kSteps]);
-        else a[t % kSteps] = x.k[i][t];
+        if (F8) decode16(kreg[i][t], scale_of(ke[i]), a[(2 * t) % kSteps], a[(2 * t + 1) % kSteps]);
+        else a[t % kSteps] = kreg[i][t];
       }
 #pragma unroll
       for (int t = 0; t < kSteps; ++t)
         s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a[t]), qf[t], s[i], 0, 0, 0);
-      const int lim = (x.live >> i) & 1 ? end - j0 - 16 * i - 4 * g : 0;
+      if (F8) __builtin_amdgcn_sched_barrier(0);  // one block's decoded keys in registers
+    }
+    if (more) load_k(j + 128);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e >= lim) s[i][e] = -INFINITY;
-    }
+        if (4 * g + e >= live[i]) s[i][e] = -INFINITY;
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
@@ -398,139 +405,157 @@ __global__ void __launch_bounds__(256) token_kernel(TokenArgs p) {
     l_run = fmaf(l_run, alpha, sum);
     const u32x4 pb = u32x4{pack_bf16x2(pr[0], pr[1]), pack_bf16x2(pr[2], pr[3]),
                            pack_bf16x2(pr[4], pr[5]), pack_bf16x2(pr[6], pr[7])};
+    // V into LDS, zero where there is no key
+#pragma unroll
+    for (int u = 0; u < kVLoads; ++u) {
+      const int row = kVRows * u + vr;
+      const bool ok = (row & 15) < live[kVRows * u < 16 ? 0 : 1];
+      lds_u8* const to = mine + row * kPitch;
+      const int ch = vd / 8, sw = swz_v<D>(row);
+      const u32x4 none = u32x4{0, 0, 0, 0};
+      if (F8) {
+        u32x4 x, y;
+        decode16(vreg[u], scale_of(ve[u]), x, y);
+        *reinterpret_cast<lds_u32x4*>(to + ((ch ^ sw) << 4)) = ok ? x : none;
+        *reinterpret_cast<lds_u32x4*>(to + (((ch + 1) ^ sw) << 4)) = ok ? y : none;
+      } else {
+        *reinterpret_cast<lds_u32x4*>(to + ((ch ^ sw) << 4)) = ok ? vreg[u] : none;
+      }
+    }
+    if (more) load_v(j + 128);
     asm volatile("" ::: "memory");  // the V rows are written before they are read
 #pragma unroll
     for (int db = 0; db < kDB; ++db) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[db][e] *= alpha;
-      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(mine + tr[db]));
-      const i16x4 up =
-          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(mine + tr[db] + 16 * kPitch));
+      const lds_u8* const x = mine + (tr ^ (32 * db));
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)x);
+      const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(x + 16 * kPitch));
       const bf16x8 a =
           __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
       o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, as_bf16x8(pb), o[db], 0, 0, 0);
+      if ((db & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // not all of V^T in registers at once
     }
     asm volatile("" ::: "memory");  // and read before the next tile's are written
-  };
-
-  Loaded x[2];
-  int j = begin + 32 * wave;
-  if (p.tab.pages > 0) {
-    if (j < end) load(j, x[0]);
-    while (j < end) {
-      if (j + 128 < end) load(j + 128, x[1]);
-      tile(j, x[0]);
-      j += 128;
-      if (j >= end) break;
-      if (j + 128 < end) load(j + 128, x[0]);
-      tile(j, x[1]);
-      j += 128;
-    }
   }
 
-  // The four waves' sums, at the largest of their references
+  // The four waves' sums, at the largest of their references, by way of LDS: O^T
+  // of lane (n, g) is head-dims 16 db + 4 g .. + 3 of query head n.
   l_run = over_groups<false>(l_run);
   if (g == 0) {
     red_m[wave][n] = m_run;
     red_l[wave][n] = l_run;
   }
   __syncthreads();
-  float m = -INFINITY;
+  {
+    float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][n]);
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][n]);
+    const float f = __builtin_amdgcn_exp2f(m_run - (m == -INFINITY ? 0.f : m));
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = f == 0.f ? 0.f : o[db][e] * f;
+      *reinterpret_cast<lds_f32x4*>((lds_u8*)vt + ((wave * 16 + n) * (D / 4) + ((4 * db + g) ^ n)) * 16) = y;
+    }
+  }
+  __syncthreads();
+  // 16 threads a query head, D / 64 times four head-dims each
+  const int qn = tid >> 4;
+  if (qn >= nq) return;
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][qn]);
   const float mu = m == -INFINITY ? 0.f : m;
-  const float mine_f = __builtin_amdgcn_exp2f(m_run - mu);
-  // O^T of lane (n, g): head-dims 16 db + 4 g .. + 3 of query head n. Into LDS
-  // (floats) a half of the waves at a time: 2 x 16 x D x 4 bytes fit the V tiles.
-  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  lds_f32x4* const box = reinterpret_cast<lds_f32x4*>((lds_u8*)vt);
-  for (int from = 2; from >= 1; from >>= 1) {
-    // waves from .. 2 from - 1 hand over to waves 0 .. from - 1
-    if (wave >= from && wave < 2 * from) {
-      const float f = from == 2 ? mine_f : 1.f;
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        f32x4 y;
+  for (int w = 0; w < 4; ++w) l += red_l[w][qn] * __builtin_amdgcn_exp2f(red_m[w][qn] - mu);
+  const int hq = head * p.group + g0 + qn;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float* const part = p.part + (((int64_t)b * heads + hq) * p.n_split + split) * (D + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = f == 0.f ? 0.f : o[db][e] * f;
-        box[((wave - from) * kDB + db) * 64 + lane] = y;
-      }
-    }
-    __syncthreads();
-    if (wave < from) {
-      const float f = from == 2 ? mine_f : 1.f;
+  for (int i = 0; i < D / 64; ++i) {
+    const int ch = 16 * i + (tid & 15);
+    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        const f32x4 y = box[(wave * kDB + db) * 64 + lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[db][e] = (f == 0.f ? 0.f : o[db][e] * f) + y[e];
-      }
-    }
-    __syncthreads();
+    for (int w = 0; w < 4; ++w)
+      y += *reinterpret_cast<const lds_f32x4*>((lds_u8*)vt + ((w * 16 + qn) * (D / 4) + (ch ^ qn)) * 16);
+    if (p.n_split == 1)
+      *reinterpret_cast<u32x2*>(p.out + b * p.os + hq * p.oh + 4 * ch) =
+          u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+    else
+      *reinterpret_cast<f32x4*>(part + 4 * ch) = y;
   }
-  if (wave != 0 || n >= nq) return;
-  float l = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) l += red_l[w][n] * __builtin_amdgcn_exp2f(red_m[w][n] - mu);
-  const int hq = head * p.group + g0 + n;
-  if (p.n_split == 1) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* to = p.out + b * p.os + hq * p.oh + 4 * g;
-#pragma unroll
-    for (int db = 0; db < kDB; ++db)
-      *reinterpret_cast<u32x2*>(to + 16 * db) =
-          u32x2{pack_bf16x2(o[db][0] * inv, o[db][1] * inv), pack_bf16x2(o[db][2] * inv, o[db][3] * inv)};
-    if (g == 0 && p.lse != nullptr)
+  if ((tid & 15) == 0) {
+    if (p.n_split > 1) {
+      part[D] = m;
+      part[D + 1] = l;
+    } else if (p.lse != nullptr) {
       p.lse[(int64_t)b * heads + hq] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-    return;
-  }
-  float* to = p.part + (((int64_t)b * heads + hq) * p.n_split + split) * (D + 4);
-#pragma unroll
-  for (int db = 0; db < kDB; ++db) *reinterpret_cast<f32x4*>(to + 16 * db + 4 * g) = o[db];
-  if (g == 0) {
-    to[D] = m;
-    to[D + 1] = l;
+    }
   }
 }
 
-// The parts of a row joined: wave = (sequence, query head), a lane D / 64
-// head-dims of it.
-template <int D>
-__global__ void __launch_bounds__(256) join_kernel(TokenArgs p) {
+// The parts of a row joined: workgroup = (sequence, query head), a wave every
+// W-th part, a lane D / 64 head-dims of it. Two passes over the references, as
+// the weights need their maximum. W is 2 for up to 32 parts, 8 beyond
+// (224 rows of 128 parts: 67 us with one wave, 18).
+template <int D, int W>
+__global__ void __launch_bounds__(64 * W) join_kernel(TokenArgs p) {
+  __shared__ float box[W][D + 2];
   const int heads = p.n_kv * p.group;
-  const int lane = threadIdx.x & 63;
-  const int hq = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), b = blockIdx.y;
-  if (hq >= heads) return;
-  const int capacity = (int)min((int64_t)p.tab.width << p.tab.shift, (int64_t)0x7fffffff);
-  const int len = min(max(p.lengths[b], 0), capacity);
-  const int n = min(max((len + p.chunk - 1) / p.chunk, 1), p.n_split);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hq = blockIdx.x, b = blockIdx.y;
+  const int n = min(max((length_of(p, b) + p.chunk - 1) / p.chunk, 1), p.n_split);
   const float* part = p.part + ((int64_t)b * heads + hq) * p.n_split * (D + 4);
+  // this wave's parts: wave, wave + W, ..; lane i has the i-th one's reference
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, part[i * (D + 4) + D]);
+  for (int i = wave + W * lane; i < n; i += 64 * W) m = fmaxf(m, part[(int64_t)i * (D + 4) + D]);
   m = wave_reduce<true>(m);
   const float mu = m == -INFINITY ? 0.f : m;
   float l = 0.f, acc[D / 64] = {};
-  for (int i0 = 0; i0 < n; i0 += 64) {
+  for (int i0 = wave; i0 < n; i0 += 64 * W) {
+    const int mine = i0 + W * lane;
     float w = 0.f;
-    if (i0 + lane < n) {
-      const float* x = part + (i0 + lane) * (D + 4) + D;
+    if (mine < n) {
+      const float* x = part + (int64_t)mine * (D + 4) + D;
       w = __builtin_amdgcn_exp2f(x[0] - mu);
       l = fmaf(w, x[1], l);
     }
-    for (int i = 0; i < min(64, n - i0); ++i) {
+    const int count = min(64, (n - i0 + W - 1) / W);
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
       const float wi = __shfl(w, i);
-      if (wi == 0.f) continue;
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e)
-        acc[e] = fmaf(wi, part[(i0 + i) * (D + 4) + lane + 64 * e], acc[e]);
+      for (int e = 0; e < D / 64; ++e) {
+        const float x = part[(int64_t)(i0 + W * i) * (D + 4) + lane + 64 * e];
+        acc[e] = wi == 0.f ? acc[e] : fmaf(wi, x, acc[e]);
+      }
     }
   }
   l = wave_reduce<false>(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e)
-    p.out[b * p.os + hq * p.oh + lane + 64 * e] = (uint16_t)f32_to_bf16(acc[e] * inv);
-  if (lane == 0 && p.lse != nullptr)
+  for (int e = 0; e < D / 64; ++e) box[wave][lane + 64 * e] = acc[e];
+  if (lane == 0) {
+    box[wave][D] = m;
+    box[wave][D + 1] = l;
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) m = fmaxf(m, box[w][D]);
+  float y = 0.f;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float f = __builtin_amdgcn_exp2f(box[w][D] - (m == -INFINITY ? 0.f : m));
+    l = fmaf(f, box[w][D + 1], l);
+    y = f == 0.f ? y : fmaf(f, box[w][d], y);
+  }
+  p.out[b * p.os + hq * p.oh + d] = (uint16_t)f32_to_bf16(l == 0.f ? 0.f : y / l);
+  if (d == 0 && p.lse != nullptr)
     p.lse[(int64_t)b * heads + hq] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
@@ -667,11 +692,15 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
   VEDA_REQUIRE(n_seq >= 0 && n_seq <= 65535, "paged_fwd: at most 65535 sequences, got %lld",
                (long long)n_seq);
   VEDA_REQUIRE(width * page < (1ll << 31), "paged_fwd: a table row holds 2^31 keys or more");
+  // a page's rows are addressed with 32-bit byte offsets
+  VEDA_REQUIRE(stride_s >= 0 && exp_stride_s >= 0 && stride_s < (1 << 22) && exp_stride_s < (1 << 22),
+               "paged_fwd: row stride of the cache negative or too large");
   VEDA_REQUIRE(scale > 0.f && scale < INFINITY, "paged_fwd: scale must be positive and finite");
   VEDA_REQUIRE(whole(q, 8, q_stride_s, q_stride_h, 0) && whole(out, 8, o_stride_s, o_stride_h, 0),
                "paged_fwd: q and out rows must be 16-byte aligned");
-  VEDA_REQUIRE(chunk >= 32 && chunk % 32 == 0 && chunk < (1ll << 30),
-               "paged_fwd: chunk must be a multiple of 32, got %lld", (long long)chunk);
+  VEDA_REQUIRE(chunk >= page && chunk % page == 0 && chunk % 32 == 0 && chunk <= 64 * page,
+               "paged_fwd: chunk must be a multiple of 32 and 1 to 64 whole pages, got %lld",
+               (long long)chunk);
   if (n_seq == 0) return VEDA_OK;
   const int64_t group = n_heads / n_kv_heads, capacity = width * page;
   const int64_t n_split = capacity > chunk ? (capacity + chunk - 1) / chunk : 1;
@@ -705,9 +734,14 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
   }
   if (n_split > 1) {
     if (int rc = check_launch("veda_paged_fwd")) return rc;
-    const dim3 jgrid((unsigned)((n_heads + 3) / 4), (unsigned)n_seq);
-    if (head_dim == 128) join_kernel<128><<<jgrid, 256, 0, s>>>(p);
-    else join_kernel<64><<<jgrid, 256, 0, s>>>(p);
+    const dim3 jgrid((unsigned)n_heads, (unsigned)n_seq);
+    if (head_dim == 128) {
+      if (n_split <= 32) join_kernel<128, 2><<<jgrid, 128, 0, s>>>(p);
+      else join_kernel<128, 8><<<jgrid, 512, 0, s>>>(p);
+    } else {
+      if (n_split <= 32) join_kernel<64, 2><<<jgrid, 128, 0, s>>>(p);
+      else join_kernel<64, 8><<<jgrid, 512, 0, s>>>(p);
+    }
   }
   return check_launch("veda_paged_fwd");
 }

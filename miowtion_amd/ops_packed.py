@@ -78,6 +78,23 @@ def _check_packed(q, k, v, cu_q, cu_k, scale):
         _ints('cu_k', cu_k, n, dev), n - 1]
 
 
+def _key_splits(q_rows: int, k_rows: int, n_seq: int, heads: int, kv_heads: int) -> int:
+    """Workgroups that share the keys of 128 query rows: enough to fill the GPU
+    (512 are resident; a quarter more where the sequences are many times as long
+    as their queries, and end unevenly), of fifteen steps of 64 keys at least
+    where half of the sequences hold all of the keys. A split's sums cost 8 bytes
+    of traffic for each of its 32-bit values, so splits past that cost more than
+    they give. Times in us with 1, 2, 4, 8 and 16 splits: 2 x 16 queries of 16
+    heads over 52,768 keys 416, 220, 119, 70, 48; 512 of 32 over 8,192: 116, 82,
+    82, 94, 122; 4 x 512 of 32 (head_dim 64) over 21,388: 131, 117, 125, 147, 204;
+    whole prompts of 1,024, 1,000, 900 and 800 tokens, 8 heads: 26, 34, 43, 67, 129."""
+    tiles = max(q_rows * heads // TILE, min(n_seq, q_rows) * kv_heads, 1)
+    want = 640 if 4 * q_rows <= k_rows else 512
+    if tiles >= want or n_seq == 0:
+        return 1
+    return max(min(-(-want // tiles), k_rows // -(-n_seq // 2) // 960, 32), 1)
+
+
 @_custom_op('veda::packed_fwd', mutates_args=())
 def packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                cu_k: torch.Tensor, causal: bool, scale: float, return_lse: bool) -> list[torch.Tensor]:
@@ -85,8 +102,14 @@ def packed_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Te
     dev, (rows, heads, d), tensors, sizes = _check_packed(q, k, v, cu_q, cu_k, scale)
     out = q.new_empty((rows, heads, d))
     lse = q.new_empty((rows, heads), dtype=_F32) if return_lse else None
-    _launch('veda_packed_fwd', dev, *tensors, *sizes, causal, scale, out.data_ptr(), heads * d, d,
-            lse.data_ptr() if return_lse else None)
+    n_split = _key_splits(rows, sizes[1], sizes[-1], heads, sizes[3])
+    work, nbytes = None, 0
+    if n_split > 1:
+        nbytes = 4 * n_split * rows * heads * (d + 2)
+        work = q.new_empty(nbytes // 4, dtype=_F32)
+    _launch('veda_packed_fwd', dev, *tensors, *sizes, causal, scale, n_split, out.data_ptr(),
+            heads * d, d, lse.data_ptr() if return_lse else None,
+            None if work is None else work.data_ptr(), nbytes)
     return [out, lse] if return_lse else [out]
 
 
@@ -219,11 +242,18 @@ def _(k_pages, v_pages, k_exp, v_exp, cu, table, rows):
     return [k_pages.new_empty(rows, *k_pages.shape[2:], dtype=torch.bfloat16) for _ in range(2)]
 
 
-def _chunk(n_seq: int, kv_heads: int, group: int, capacity: int) -> int:
-    """Keys of a workgroup of paged_fwd."""
+def _chunk(n_seq: int, kv_heads: int, group: int, capacity: int, page: int) -> int:
+    """Keys of a workgroup of paged_fwd, from how far the table reaches (the
+    lengths are on the GPU)."""
     groups = n_seq * kv_heads * -(-group // 16)
-    even = -(-(capacity * groups // 1024) // 128) * 128
-    return min(max(even, 128), 1024)
+    if capacity <= 1024 and groups >= 256:
+        chunk = capacity  # enough workgroups as it is: nothing to join
+    else:
+        chunk = min(max(capacity // 24, 256), 1024)
+        if groups * -(-capacity // chunk) < 512:  # few workgroups: smaller ones, to a point
+            chunk = max(capacity * groups // 512, 128 if capacity <= 4096 else 256)
+    unit = max(page, 128)
+    return min(-(-chunk // unit) * unit, 64 * page)
 
 
 @_custom_op('veda::paged_fwd', mutates_args=())
@@ -241,7 +271,7 @@ def paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if table.shape[0] != n:
         raise ValueError(f'table has {table.shape[0]} sequences, q {n}')
     capacity = table.shape[1] * k_pages.shape[1]
-    chunk = _chunk(n, kv, heads // kv, capacity)
+    chunk = _chunk(n, kv, heads // kv, capacity, k_pages.shape[1])
     n_split = -(-capacity // chunk)
     out = q.new_empty((n, heads, d))
     lse = q.new_empty((n, heads), dtype=_F32) if return_lse else None

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from miowtion_amd import kernels
+from miowtion_amd import kernels, ops_packed
 from tests import packed_reference as pr
 
 pytestmark = pytest.mark.gpu
@@ -57,6 +57,45 @@ def test_forward(case):
     pr.check(lse, ref, 'lse')
     again = kernels.packed_attention(q, k, v, cu_q, None if lens_k == lens_q else cu_k, causal=causal)
     assert torch.equal(out, again)
+
+
+SPLIT = [
+    # few rows against many keys: several workgroups share a row's keys
+    ([5, 0, 130], [4000, 2100, 3001], 8, 2, 128, True),
+    ([5, 0, 130], [4000, 2100, 3001], 4, 4, 64, False),
+    ([1], [5000], 6, 1, 64, True),
+    ([2500], None, 2, 1, 128, True),
+    ([700, 40, 1], [700, 6000, 30], 2, 2, 64, True),
+    ([3000, 2], [2000, 1], 1, 1, 128, True),         # rows that see nothing
+]
+
+
+@pytest.mark.parametrize('case', SPLIT, ids=lambda c: f'{len(c[0])}x{max(c[0])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}')
+def test_keys_shared_by_workgroups(case):
+    lens_q, lens_k, heads, kv, d, causal = case
+    lens_k = lens_k or lens_q
+    print(f'packed forward, keys split {case}', flush=True)
+    assert ops_packed._key_splits(sum(lens_q), sum(lens_k), len(lens_q), heads, kv) > 1
+    q, k, v = _inputs(lens_q, lens_k, heads, kv, d, seed=2)
+    cu_q, cu_k = pr.offsets(lens_q), pr.offsets(lens_k)
+    out, lse = kernels.packed_attention(q, k, v, cu_q, cu_k, causal=causal, return_lse=True)
+    ref = pr.attend(q, k, v, lens_q, lens_k, causal)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+    assert torch.equal(out, kernels.packed_attention(q, k, v, cu_q, cu_k, causal=causal))
+    # a value that is not finite in the middle of the first sequence's keys
+    at = lens_k[0] // 2
+    v[at, 0, 3] = math.nan
+    got = kernels.packed_attention(q, k, v, cu_q, cu_k, causal=causal)
+    sees = torch.zeros(sum(lens_q), dtype=torch.bool)
+    first = lens_q[0]
+    i = torch.arange(first)
+    sees[:first] = (i + lens_k[0] - lens_q[0] >= at) if causal else True
+    group = heads // kv
+    assert torch.isnan(got[sees][:, :group, 3]).all()
+    rest = got.clone()
+    rest[:, :group, 3] = torch.where(sees[:, None].cuda(), ref['out'][:, :group, 3].to(got.dtype), got[:, :group, 3])
+    pr.check(rest, ref, 'out')
 
 
 def test_scale_and_large_scores():
