@@ -259,6 +259,9 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int end = 64 * n_steps;
   const int limit = min(max((real ? visible_keys(p.pk, sp, r) : last) - 64 * from, 0), end);
   const int n_plain = min(max(visible_keys(p.pk, sp, r0) - 64 * from, 0), end) >> 6;  // seen whole by every row
+  // keys that every row of the wave sees (its rows see more and more)
+  const int wave_all = __builtin_amdgcn_readfirstlane(
+      min(max((r0 + 32 * wave < rows ? visible_keys(p.pk, sp, r0 + 32 * wave) : last) - 64 * from, 0), end));
   const int nk = sp.nk - 64 * from;
   const int64_t token = sp.q0 + r / p.pk.group;
   const int64_t qhead = (int64_t)head * p.pk.group + r % p.pk.group;
@@ -333,10 +336,10 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
     };
     Next<D> next;
     stage<D, true, kSmSecond, true, kReadNext>(s0 + nxt, s0 + cur, f, c, sa, sb, pb, pa, w, hook, &next);
-    if (MASKED) mask_scores(sa, limit - 64 * (u + 1), hi);
+    if (MASKED && 64 * (u + 1) + 32 > wave_all) mask_scores(sa, limit - 64 * (u + 1), hi);
     stage<D, true, kSmFirst, true, kTakeNext>(s0 + nxt + kSub, s0 + cur + kSub, f, c, sb, sa, pa, pb, w,
                                               NoHook{}, &next);
-    if (MASKED) mask_scores(sb, limit - 64 * (u + 1) - 32, hi);
+    if (MASKED && 64 * (u + 1) + 64 > wave_all) mask_scores(sb, limit - 64 * (u + 1) - 32, hi);
   };
   if (n_steps > 0) {
     const Src k0 = src_of(kbase, p.ks, 0, false, true), k1 = src_of(kbase, p.ks, 1, false, true);
@@ -456,10 +459,12 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(FwdArgs p) {
   if (row >= all_rows) return;
   const f32x2* ml = reinterpret_cast<const f32x2*>(p.part + p.n_split * all_rows * D) + row;
   float m = -INFINITY;
+#pragma unroll 4
   for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, ml[s * all_rows][0]);
   const float mu = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < p.n_split; ++s) {
     const f32x2 x = ml[s * all_rows];
     const float w = __builtin_amdgcn_exp2f(x[0] - mu);
@@ -493,8 +498,8 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
                "packed_fwd: %lld query heads are no multiple of %lld key heads", (long long)n_heads,
                (long long)n_kv_heads);
   VEDA_REQUIRE(q_rows >= 0 && k_rows >= 0 && n_seq >= 0, "packed_fwd: negative size");
-  VEDA_REQUIRE(q_rows * n_heads < (1ll << 31) && k_rows < (1ll << 31) && n_seq < (1 << 20),
-               "packed_fwd: q_rows x heads or k_rows of 2^31 or more, or 2^20 sequences");
+  VEDA_REQUIRE(q_rows * n_heads <= 0x7fffff00 && k_rows <= 0x7fffff00 && n_seq < (1 << 20),
+               "packed_fwd: q_rows x heads or k_rows past 2^31 - 256, or 2^20 sequences");
   VEDA_REQUIRE(scale > 0.f && scale < INFINITY, "packed_fwd: scale must be positive and finite");
   VEDA_REQUIRE(rows16(q, q_stride_s, q_stride_h) && rows16(k, k_stride_s, k_stride_h) &&
                    rows16(v, v_stride_s, v_stride_h) && rows16(out, o_stride_s, o_stride_h),

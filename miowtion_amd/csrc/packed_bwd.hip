@@ -335,9 +335,14 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   const uint16_t* qhead = p.q + (int64_t)sp.q0 * p.qs + (int64_t)head * group * p.qh;
   const uint16_t* dhead = p.dout + (int64_t)sp.q0 * p.dos + (int64_t)head * group * p.doh;
 
+  // The steps' rows are loaded in turn: t0, rem are the next step's first token
+  // and head. Row x from there is token x / group by a product with 2^32 / group
+  // (exact: x < 64 + group, and x group < 2^32).
+  int t0 = (int)((int64_t)64 * u0 / group), rem = (int)((int64_t)64 * u0 - (int64_t)t0 * group);
+  const int t_step = 64 / group, r_step = 64 - t_step * group;
+  const uint32_t per_group = 0xffffffffu / (uint32_t)group + 1;  // 0 for a group of one
   auto load_step = [&](int u, lds_u8* dst) {
     const int lane = lane_anew();
-    const int t0 = 64 * u / group, rem = 64 * u - t0 * group;  // the step's first token and head
     const char* qb = reinterpret_cast<const char*>(qhead + (int64_t)t0 * p.qs);
     const char* db = reinterpret_cast<const char*>(dhead + (int64_t)t0 * p.dos);
 #pragma unroll
@@ -345,11 +350,17 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
       const int seg = T::kSegs * wave + s;
       const int row = seg * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
       const uint32_t x = (uint32_t)(min(row, rows - 1 - 64 * u) + rem);
-      const uint32_t t = x / (uint32_t)group, g = x - t * (uint32_t)group;
+      const uint32_t t = group == 1 ? x : __umulhi(x, per_group), g = x - t * (uint32_t)group;
       const uint32_t ch = (uint32_t)((pos ^ swz_both<D>(row)) << 4);
       dma16(qb, t * (uint32_t)(2 * p.qs) + g * (uint32_t)(2 * p.qh) + ch, dst + seg * 1024);
       dma16(db, t * (uint32_t)(2 * p.dos) + g * (uint32_t)(2 * p.doh) + ch,
             dst + T::kBytes + seg * 1024);
+    }
+    t0 += t_step;
+    rem += r_step;
+    if (rem >= group) {
+      rem -= group;
+      ++t0;
     }
     if (wave == 0)
       dma16(reinterpret_cast<const char*>(recs + (int64_t)u * kRecFloats), (uint32_t)((lane & 31) * 16),
@@ -522,8 +533,8 @@ extern "C" int veda_packed_bwd(
                "packed_bwd: %lld query heads are no multiple of %lld key heads", (long long)n_heads,
                (long long)n_kv_heads);
   VEDA_REQUIRE(q_rows >= 0 && k_rows >= 0 && n_seq >= 0, "packed_bwd: negative size");
-  VEDA_REQUIRE(q_rows * n_heads < (1ll << 31) && k_rows < (1ll << 31) && n_seq < (1 << 20),
-               "packed_bwd: q_rows x heads or k_rows of 2^31 or more, or 2^20 sequences");
+  VEDA_REQUIRE(q_rows * n_heads <= 0x7fffff00 && k_rows <= 0x7fffff00 && n_seq < (1 << 20),
+               "packed_bwd: q_rows x heads or k_rows past 2^31 - 256, or 2^20 sequences");
   VEDA_REQUIRE(scale > 0.f && scale < INFINITY, "packed_bwd: scale must be positive and finite");
   VEDA_REQUIRE(rows16(q, q_stride_s, q_stride_h) && rows16(k, k_stride_s, k_stride_h) &&
                    rows16(v, v_stride_s, v_stride_h) && rows16(out, o_stride_s, o_stride_h) &&
@@ -537,6 +548,7 @@ extern "C" int veda_packed_bwd(
   BwdArgs p{};
   p.pk = Packing{cu_q, cu_k, (int32_t)n_seq, (int32_t)q_rows, (int32_t)k_rows, (int32_t)n_kv_heads,
                  (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0};
+  VEDA_REQUIRE(p.pk.group <= 65000, "packed_bwd: at most 65000 query heads to a key head");
   VEDA_REQUIRE(p.pk.group <= 64 || (q_stride_h * p.pk.group < (1 << 30) &&
                                     do_stride_h * p.pk.group < (1 << 30)),
                "packed_bwd: the heads of a group are too far apart");
