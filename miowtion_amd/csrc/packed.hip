@@ -522,8 +522,12 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
   p.lse = lse;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int64_t slots = slots_of(q_rows, p.pk.group, n_seq);
-  VEDA_REQUIRE(n_split >= 1 && n_split <= 64 && slots * n_kv_heads * n_split < (1ll << 31),
-               "packed_fwd: n_split %lld outside [1, 64], or too many tiles", (long long)n_split);
+  VEDA_REQUIRE(n_split >= 1 && n_split <= 64, "packed_fwd: n_split %lld outside [1, 64]",
+               (long long)n_split);
+  // a launch holds less than 2^32 threads
+  VEDA_REQUIRE(slots * n_kv_heads * n_split < (1 << 24) &&
+                   (n_split == 1 || q_rows * n_heads < (1 << 27)),
+               "packed_fwd: too many rows for one launch");
   const int64_t need = n_split == 1 ? 0 : n_split * q_rows * n_heads * (head_dim + 2) * 4;
   VEDA_REQUIRE(need == 0 || (workspace != nullptr && rows16(workspace, 0, 0) && workspace_bytes >= need),
                "packed_fwd: workspace needs %lld bytes (16-byte aligned), got %lld", (long long)need,

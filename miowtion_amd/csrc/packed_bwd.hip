@@ -553,11 +553,13 @@ extern "C" int veda_packed_bwd(
                                     do_stride_h * p.pk.group < (1 << 30)),
                "packed_bwd: the heads of a group are too far apart");
   const int64_t q_slots = slots_of(q_rows, p.pk.group, n_seq), k_slots = slots_of(k_rows, 1, n_seq);
-  VEDA_REQUIRE(q_slots * n_kv_heads < (1ll << 31) && k_slots * n_kv_heads < (1ll << 31),
-               "packed_bwd: too many tiles");
-  VEDA_REQUIRE(n_split >= 1 && n_split <= 64 && k_slots * n_kv_heads * n_split < (1ll << 31),
-               "packed_bwd: n_split %lld outside [1, 64], or too many tiles", (long long)n_split);
+  VEDA_REQUIRE(n_split >= 1 && n_split <= 64, "packed_bwd: n_split %lld outside [1, 64]",
+               (long long)n_split);
   const int64_t n_out = k_rows * n_kv_heads * head_dim;
+  // a launch holds less than 2^32 threads
+  VEDA_REQUIRE(q_slots * n_kv_heads < (1 << 24) && k_slots * n_kv_heads * n_split < (1 << 24) &&
+                   (n_split == 1 || n_out < (1ll << 33)),
+               "packed_bwd: too many rows for one launch");
   const int64_t rec_bytes = q_slots * n_kv_heads * 2 * kRecBytes;
   const int64_t need = rec_bytes + (n_split > 1 ? 2 * n_split * n_out * 4 : 0);
   VEDA_REQUIRE(workspace != nullptr && rows16(workspace, 0, 0) && workspace_bytes >= need,

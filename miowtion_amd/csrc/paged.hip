@@ -263,8 +263,7 @@ __device__ __forceinline__ float over_groups(float v) {
 }
 
 __device__ __forceinline__ int length_of(const TokenArgs& p, int b) {
-  const int capacity = (int)min((int64_t)p.tab.width << p.tab.shift, (int64_t)0x7fffffff);
-  return min(max(p.lengths[b], 0), capacity);
+  return min(max(p.lengths[b], 0), p.tab.width << p.tab.shift);
 }
 
 template <int D, bool F8>
@@ -664,8 +663,9 @@ extern "C" int veda_cache_append(const void* k, int64_t k_stride_s, int64_t k_st
   p.vp = pages_of(v_pages, stride_p, stride_s, stride_h, v_exp, exp_stride_p, exp_stride_s, exp_stride_h);
   if (int rc = check_cache("cache_append", head_dim, n_kv_heads, n_pages, page, width, e4m3, p.kp, p.vp))
     return rc;
-  VEDA_REQUIRE(rows >= 0 && rows < (1ll << 31) && n_seq >= 0 && n_seq < (1 << 20),
-               "cache_append: rows or sequences out of range");
+  // (a wave a row, and a launch holds less than 2^32 threads)
+  VEDA_REQUIRE(rows >= 0 && rows < (1 << 26) && n_seq >= 0 && n_seq < (1 << 20),
+               "cache_append: 2^26 rows or 2^20 sequences, or negative");
   VEDA_REQUIRE(whole(k, 8, k_stride_s, k_stride_h, 0) && whole(v, 8, v_stride_s, v_stride_h, 0),
                "cache_append: k and v rows must be 16-byte aligned");
   if (rows == 0 || n_seq == 0) return VEDA_OK;
@@ -703,8 +703,8 @@ extern "C" int veda_cache_gather(const void* k_pages, const void* v_pages, int64
   p.vp = pages_of(v_pages, stride_p, stride_s, stride_h, v_exp, exp_stride_p, exp_stride_s, exp_stride_h);
   if (int rc = check_cache("cache_gather", head_dim, n_kv_heads, n_pages, page, width, e4m3, p.kp, p.vp))
     return rc;
-  VEDA_REQUIRE(rows >= 0 && rows < (1ll << 31) && n_seq >= 0 && n_seq < (1 << 20),
-               "cache_gather: rows or sequences out of range");
+  VEDA_REQUIRE(rows >= 0 && rows < (1 << 26) && n_seq >= 0 && n_seq < (1 << 20),
+               "cache_gather: 2^26 rows or 2^20 sequences, or negative");
   VEDA_REQUIRE(whole(k, 8, 0, 0, 0) && whole(v, 8, 0, 0, 0), "cache_gather: k and v must be 16-byte aligned");
   if (rows == 0) return VEDA_OK;
   p.tab = table_of(table, table_ld, width, n_pages, page);
@@ -746,7 +746,7 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
                (long long)n_kv_heads);
   VEDA_REQUIRE(n_seq >= 0 && n_seq <= 65535, "paged_fwd: at most 65535 sequences, got %lld",
                (long long)n_seq);
-  VEDA_REQUIRE(width * page < (1ll << 31), "paged_fwd: a table row holds 2^31 keys or more");
+  VEDA_REQUIRE(width * page <= 0x7fff0000, "paged_fwd: a table row holds nearly 2^31 keys");
   // a page's rows are addressed with 32-bit byte offsets
   VEDA_REQUIRE(stride_s >= 0 && exp_stride_s >= 0 && stride_s < (1 << 22) && exp_stride_s < (1 << 22),
                "paged_fwd: row stride of the cache negative or too large");
@@ -764,7 +764,9 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
                              workspace != nullptr && workspace_bytes >= need),
                "paged_fwd: workspace needs %lld bytes (16-byte aligned), got %lld", (long long)need,
                (long long)workspace_bytes);
-  VEDA_REQUIRE(n_split * n_kv_heads < (1ll << 31) && group <= 16 * 65535, "paged_fwd: too many heads");
+  VEDA_REQUIRE(n_split * n_kv_heads < (1 << 24) && group <= 16 * 65535 && n_heads * n_seq < (1 << 26) &&
+                   n_heads < (1 << 23),
+               "paged_fwd: too many heads for one launch");
   p.q = static_cast<const uint16_t*>(q);
   p.qs = q_stride_s; p.qh = q_stride_h;
   p.tab = table_of(table, table_ld, width, n_pages, page);
