@@ -662,7 +662,7 @@ int veda_cache_gather(const void* k_pages, const void* v_pages,
  * first lengths[b] positions of sequence b (clamped to the table's width;
  * positions of no row draw no weight). out [n_seq, n_heads, D] bf16, lse fp32
  * [n_seq, n_heads] contiguous or NULL; out = 0 and lse = -inf without a key.
- * chunk: keys of a workgroup, a multiple of 32 and 1 to 64 whole pages. With n_split = ceil(width *
+ * chunk: keys of a workgroup, a multiple of 32 and 1 to 128 whole pages. With n_split = ceil(width *
  * page / chunk) above 1, workspace holds n_seq * n_heads * n_split * (D + 4)
  * floats, 16-byte aligned.
  */

@@ -12,6 +12,8 @@
 // Position i of sequence b lies in page table[b][i / page], row i % page. A
 // page number outside the cache, or a position past the table, is no row: it is
 // not written, reads as zeros and draws no weight.
+#include <type_traits>
+
 #include "veda_pipeline.h"
 
 namespace veda {
@@ -219,9 +221,9 @@ __global__ void __launch_bounds__(256) gather_cache_kernel(GatherArgs p) {
 
 // ---------------------------------------------------------------------------
 // One new token of every sequence. Workgroup = (sequence, key head, up to 16 of
-// its query heads, `chunk` keys of the sequence), 4 waves; each wave has tiles
-// of 32 keys of its own, every fourth of the chunk, and nothing waits for
-// another wave until the end. With v_mfma_f32_16x16x32_bf16 (A[i][k] in lane
+// its query heads, `chunk` keys of the sequence), W waves (4, or 8 where a whole
+// sequence is one chunk); each wave has tiles of 32 keys of its own, every W-th
+// of the chunk, and nothing waits for another wave until the end. With v_mfma_f32_16x16x32_bf16 (A[i][k] in lane
 // i + 16 (k / 8) and B[k][j] in lane j + 16 (k / 8), element k % 8; D[i][j] in
 // lane j + 16 (i / 4), element i % 4) the scores are S^T = K Q^T: lane n + 16 g
 // holds keys 4 g .. + 3 of both 16-key blocks of query head n, which are the
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(256) gather_cache_kernel(GatherArgs p) {
 // Bound by the cache's bytes: a tile's K is asked for once the last tile's
 // scores are formed, its V once the last one's is in LDS, so a wave has a tile in
 // flight at all times in the registers of one. The chunk's page numbers are in
-// one register from the start (lane i: page i of the chunk).
+// two registers from the start (lane i: pages i and 64 + i of the chunk).
 
 struct TokenArgs {
   const uint16_t* q;
@@ -266,8 +268,9 @@ __device__ __forceinline__ int length_of(const TokenArgs& p, int b) {
   return min(max(p.lengths[b], 0), p.tab.width << p.tab.shift);
 }
 
-template <int D, bool F8>
-__global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
+template <int D, bool F8, int W>
+__global__ void __launch_bounds__(64 * W, W == 4 ? 3 : 2) token_kernel(TokenArgs p) {
+  constexpr int kStride = 32 * W;             // keys of a round of the waves
   constexpr int kPitch = 2 * D;               // a V row in LDS, bf16
   constexpr int kTileBytes = 32 * kPitch;
   constexpr int kPer = F8 ? 16 : 8;           // elements of a 16-byte load
@@ -280,8 +283,8 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   constexpr int kDB = D / 16;
   typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  __shared__ __attribute__((aligned(1024))) uint8_t vt[4 * kTileBytes];
-  __shared__ float red_m[4][16], red_l[4][16];
+  __shared__ __attribute__((aligned(1024))) uint8_t vt[W * kTileBytes];
+  __shared__ float red_m[W][16], red_l[W][16];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int n = lane & 15, g = lane >> 4;
@@ -296,13 +299,16 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   const int end = min(begin + p.chunk, len);
   const int nq = min(p.group - g0, 16);
 
-  // the chunk's pages, -1 where there is none (64 at most)
+  // the chunk's pages, -1 where there is none (128 at most)
   const int first_page = begin >> p.tab.shift;
-  int pages = -1;
+  int pages[2] = {-1, -1};
   if (begin < len) {
-    const int i = min(first_page + lane, (len - 1) >> p.tab.shift);
-    pages = p.tab.t[b * p.tab.ld + i];
-    pages = pages >= 0 && pages < p.tab.pages ? pages : -1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = min(first_page + 64 * i + lane, (len - 1) >> p.tab.shift);
+      const int g = p.tab.t[b * p.tab.ld + at];
+      pages[i] = g >= 0 && g < p.tab.pages ? g : -1;
+    }
   }
   // Q: query head n, in the order of the K loads' elements
   bf16x8 qf[kSteps];
@@ -320,7 +326,10 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   const uint8_t* const kex = F8 ? p.kp.e + head * p.kp.eh : nullptr;
   const uint8_t* const vex = F8 ? p.vp.e + head * p.vp.eh : nullptr;
   const uint32_t row_bytes = (uint32_t)(p.kp.ss * kBytes), row_exps = (uint32_t)p.kp.es;
-  auto page_at = [&](int j) { return __builtin_amdgcn_readlane(pages, (j >> p.tab.shift) - first_page); };
+  auto page_at = [&](int j) {
+    const int i = (j >> p.tab.shift) - first_page;
+    return i < 64 ? __builtin_amdgcn_readlane(pages[0], i) : __builtin_amdgcn_readlane(pages[1], i - 64);
+  };
   // Block i of 16 keys of the tile at j0 lies in one page. Past the sequence's
   // end its rows are the rest of the last page, which no row's score or
   // probability takes in.
@@ -364,8 +373,8 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
     load_k(j);
     load_v(j);
   }
-  for (; j < end; j += 128) {
-    const bool more = j + 128 < end;
+  for (; j < end; j += kStride) {
+    const bool more = j + kStride < end;
     const int live[2] = {page_at(j) >= 0 ? end - j : 0, page_at(j + 16) >= 0 ? end - j - 16 : 0};
     f32x4 s[2];
 #pragma unroll
@@ -382,7 +391,7 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
         s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a[t]), qf[t], s[i], 0, 0, 0);
       if (F8) __builtin_amdgcn_sched_barrier(0);  // one block's decoded keys in registers
     }
-    if (more) load_k(j + 128);
+    if (more) load_k(j + kStride);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
         *reinterpret_cast<lds_u32x4*>(to + ((ch ^ sw) << 4)) = ok ? vreg[u] : none;
       }
     }
-    if (more) load_v(j + 128);
+    if (more) load_v(j + kStride);
     asm volatile("" ::: "memory");  // the V rows are written before they are read
 #pragma unroll
     for (int db = 0; db < kDB; ++db) {
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
     asm volatile("" ::: "memory");  // and read before the next tile's are written
   }
 
-  // The four waves' sums, at the largest of their references, by way of LDS: O^T
+  // The waves' sums, at the largest of their references, by way of LDS: O^T
   // of lane (n, g) is head-dims 16 db + 4 g .. + 3 of query head n.
   l_run = over_groups<false>(l_run);
   if (g == 0) {
@@ -449,7 +458,7 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   {
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][n]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, red_m[w][n]);
     const float f = __builtin_amdgcn_exp2f(m_run - (m == -INFINITY ? 0.f : m));
 #pragma unroll
     for (int db = 0; db < kDB; ++db) {
@@ -465,10 +474,10 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
   if (qn >= nq) return;
   float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][qn]);
+  for (int w = 0; w < W; ++w) m = fmaxf(m, red_m[w][qn]);
   const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) l += red_l[w][qn] * __builtin_amdgcn_exp2f(red_m[w][qn] - mu);
+  for (int w = 0; w < W; ++w) l += red_l[w][qn] * __builtin_amdgcn_exp2f(red_m[w][qn] - mu);
   const int hq = head * p.group + g0 + qn;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float* const part = p.part + (((int64_t)b * heads + hq) * p.n_split + split) * (D + 4);
@@ -477,7 +486,7 @@ __global__ void __launch_bounds__(256, 3) token_kernel(TokenArgs p) {
     const int ch = 16 * i + (tid & 15);
     f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < W; ++w)
       y += *reinterpret_cast<const lds_f32x4*>((lds_u8*)vt + ((w * 16 + qn) * (D / 4) + (ch ^ qn)) * 16);
     if (p.n_split == 1)
       *reinterpret_cast<u32x2*>(p.out + b * p.os + hq * p.oh + 4 * ch) =
@@ -753,8 +762,8 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
   VEDA_REQUIRE(scale > 0.f && scale < INFINITY, "paged_fwd: scale must be positive and finite");
   VEDA_REQUIRE(whole(q, 8, q_stride_s, q_stride_h, 0) && whole(out, 8, o_stride_s, o_stride_h, 0),
                "paged_fwd: q and out rows must be 16-byte aligned");
-  VEDA_REQUIRE(chunk >= page && chunk % page == 0 && chunk % 32 == 0 && chunk <= 64 * page,
-               "paged_fwd: chunk must be a multiple of 32 and 1 to 64 whole pages, got %lld",
+  VEDA_REQUIRE(chunk >= page && chunk % page == 0 && chunk % 32 == 0 && chunk <= 128 * page,
+               "paged_fwd: chunk must be a multiple of 32 and 1 to 128 whole pages, got %lld",
                (long long)chunk);
   if (n_seq == 0) return VEDA_OK;
   const int64_t group = n_heads / n_kv_heads, capacity = width * page;
@@ -782,13 +791,19 @@ extern "C" int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_strid
   p.part = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(n_split * n_kv_heads), (unsigned)n_seq, (unsigned)((group + 15) / 16));
-  if (head_dim == 128) {
-    if (e4m3) token_kernel<128, true><<<grid, 256, 0, s>>>(p);
-    else token_kernel<128, false><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (e4m3) token_kernel<64, true><<<grid, 256, 0, s>>>(p);
-    else token_kernel<64, false><<<grid, 256, 0, s>>>(p);
-  }
+  auto launch = [&](auto d, auto f8) {
+    // eight waves where they are all that a sequence gets and the launch leaves room
+    if (n_split == 1 && capacity > 128 && grid.x * grid.y * grid.z < 256)
+      token_kernel<decltype(d)::value, decltype(f8)::value, 8><<<grid, 512, 0, s>>>(p);
+    else
+      token_kernel<decltype(d)::value, decltype(f8)::value, 4><<<grid, 256, 0, s>>>(p);
+  };
+  using D128 = std::integral_constant<int, 128>;
+  using D64 = std::integral_constant<int, 64>;
+  if (head_dim == 128 && e4m3) launch(D128{}, std::true_type{});
+  else if (head_dim == 128) launch(D128{}, std::false_type{});
+  else if (e4m3) launch(D64{}, std::true_type{});
+  else launch(D64{}, std::false_type{});
   if (n_split > 1) {
     if (int rc = check_launch("veda_paged_fwd")) return rc;
     const dim3 jgrid((unsigned)n_heads, (unsigned)n_seq);

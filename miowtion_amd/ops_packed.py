@@ -250,17 +250,20 @@ def _chunk(n_seq: int, kv_heads: int, group: int, capacity: int, page: int) -> i
     768 workgroups that are resident, long enough to hide their start and end.
     Times in us with chunks of 128, 256, 384, 512 and 1,024: 64 sequences of up to
     8,021 (8 key heads, e4m3) 56, 49, 41, 45, 49; four of about 100,000 349, 326,
-    314, 306, 289; eight of 4,096 29, 28, 27, 27, 27. Up to 1,024 keys in 256
-    workgroups or more are not split at all: 64 of 1,000, 4 key heads 22 -> 18."""
+    314, 306, 289; eight of 4,096 29, 28, 27, 27, 27. Short sequences, or not so
+    short ones in many workgroups, are not split: in a captured graph, whole and
+    in chunks of 128, bf16, 8 key heads: one of 300 7.4 and 7.2, of 600 9.8 and 7.4,
+    of 1,500 18.4 and 7.8; sixteen of 300 7.5 and 9.1, of 600 11.2 and 13.0, of
+    1,000 15.8 and 17.5 (a call by itself is 4 us of host work less)."""
     groups = n_seq * kv_heads * -(-group // 16)
-    if capacity <= 1024 and groups >= 256:
+    if capacity <= 512 or (capacity <= 1024 and groups >= 128):
         chunk = capacity
     else:
         chunk = min(max(capacity // 24, 256), 1024)
         if groups * -(-capacity // chunk) < 512:  # few workgroups: smaller ones, to a point
             chunk = max(capacity * groups // 512, 128 if capacity <= 4096 else 256)
     unit = max(page, 128)
-    return min(-(-chunk // unit) * unit, 64 * page)
+    return min(max(-(-chunk // unit), 1) * unit, 128 * page)
 
 
 @_custom_op('veda::paged_fwd', mutates_args=())
