@@ -35,6 +35,7 @@ struct FwdArgs {
                 // pairs of reference (log2) and sum of weights
   float scale_log2;
   int32_t n_slots, n_split;
+  uint32_t per_group;
 };
 
 // A row whose O came out with an infinity or a NaN, again, key by key: a key
@@ -265,11 +266,10 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int nk = sp.nk - 64 * from;
   const int64_t token = sp.q0 + r / p.pk.group;
   const int64_t qhead = (int64_t)head * p.pk.group + r % p.pk.group;
-  const uint16_t* qptr = p.q + token * p.qs + qhead * p.qh;
+  const RowLoads<D> qrows =
+      load_rows<D>(p.q + (int64_t)sp.q0 * p.qs + (int64_t)head * p.pk.group * p.qh, p.qs, p.qh, p.pk.group,
+                   p.per_group, r0 + 32 * wave, rows, lane);
   Wave<D> w;
-#pragma unroll
-  for (int s = 0; s < T::kK; ++s)
-    w.qf[s] = real ? as_bf16x8(ld16(qptr + 16 * s + 8 * hi)) : as_bf16x8(u32x4{0, 0, 0, 0});
 
   const uint16_t* kbase = p.k + (int64_t)(sp.k0 + 64 * from) * p.ks + head * p.kh;
   const uint16_t* vbase = p.v + (int64_t)(sp.k0 + 64 * from) * p.vs + head * p.vh;
@@ -347,12 +347,14 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
 #pragma unroll
     for (int s = 0; s < T::kSegs; ++s) issue(k0, s, lds0);
 #pragma unroll
-    for (int s = 0; s < T::kSegs; ++s) issue(k1, s, lds0 + kSlot);
-#pragma unroll
     for (int s = 0; s < T::kSegs; ++s) issue(v0, s, lds0 + T::kBytes);
-    VEDA_WAIT_VM(2 * T::kSegs);  // K of step 0; K of step 1 and V of step 0 may be in flight
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    // Q by way of slot 1, which K of step 1 is loaded into after the barrier
+    frags_of_rows<D>(qrows, s0 + kSlot + wave * 32 * T::kPitch, lane, w.qf);
+#pragma unroll
+    for (int s = 0; s < T::kK; ++s) asm volatile("" : : "v"(w.qf[s]));
+    sync();
+#pragma unroll
+    for (int s = 0; s < T::kSegs; ++s) issue(k1, s, lds0 + kSlot);
     stage<D, true, kNoSm, false>(s0, s0, f, c, sa, sb, pb, pa, w, NoHook{});
     stage<D, true, kNoSm, false>(s0 + kSub, s0, f, c, sb, sa, pa, pb, w, NoHook{});
     if (n_plain == 0) {
@@ -534,6 +536,7 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
                (long long)workspace_bytes);
   p.part = static_cast<float*>(workspace);
   p.n_split = (int32_t)n_split;
+  p.per_group = per_group_of((uint32_t)p.pk.group);
   p.n_slots = (int32_t)slots;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)(slots * n_kv_heads * n_split);

@@ -59,6 +59,7 @@ struct BwdArgs {
   float* part;        // [dv | dk][n_split][k_rows, n_kv, D] sums, with n_split > 1
   float scale, scale_log2;
   int32_t q_slots, k_slots, n_split;
+  uint32_t per_group;  // 2^32 / group
 };
 
 // The lane's index, formed anew at each call, so that what is derived from it
@@ -137,35 +138,48 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   const int limit = real ? visible_keys(p.pk, sp, r) : 0;
   const int n_steps = (last + 63) >> 6;
   const int n_plain = r0 + kRows <= rows ? visible_keys(p.pk, sp, r0) >> 6 : 0;
-  const int64_t token = sp.q0 + r / group;
-  const int64_t qhead = (int64_t)head * group + r % group;
   const int64_t n_heads = (int64_t)p.pk.n_kv * group;
+  lds_u8* const s0 = (lds_u8*)ring[0];
   bf16x8 qf[kQReg], dof[T::kK];
   lds_u8* const qmine = (lds_u8*)qbox + wave * 4096;
   float dot = 0.f;
-  const bf16x8 zero = as_bf16x8(u32x4{0, 0, 0, 0});
+  {
+    // Q, dO and O by way of slot 1, which is loaded into after the first barrier
+    auto rows_of = [&](const uint16_t* x, int64_t s, int64_t h) {
+      return load_rows<D>(x + (int64_t)sp.q0 * s + (int64_t)head * group * h, s, h, group, p.per_group,
+                          r0 + 32 * wave, rows, lane);
+    };
+    const RowLoads<D> a = rows_of(p.q, p.qs, p.qh), b = rows_of(p.dout, p.dos, p.doh),
+                      c = rows_of(p.o, p.os, p.oh);
+    lds_u8* const box = s0 + kSlot + wave * 32 * T::kPitch;
+    bf16x8 x[T::kK];
+    frags_of_rows<D>(a, box, lane, x);
 #pragma unroll
-  for (int s = 0; s < T::kK; ++s) {
-    const int d = 16 * s + 8 * hi;
-    const bf16x8 qx = real ? as_bf16x8(ld16(p.q + token * p.qs + qhead * p.qh + d)) : zero;
-    if (s < kQReg) qf[s] = qx;
-    else *reinterpret_cast<lds_u32x4*>(qmine + ((s - kQReg) * 64 + lane) * 16) = __builtin_bit_cast(u32x4, qx);
-    dof[s] = real ? as_bf16x8(ld16(p.dout + token * p.dos + qhead * p.doh + d)) : zero;
-    const u32x4 a = __builtin_bit_cast(u32x4, dof[s]);
-    const u32x4 b = real ? ld16(p.o + token * p.os + qhead * p.oh + d) : u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      dot = fmaf(bf16_to_f32(a[m] & 0xffffu), bf16_to_f32(b[m] & 0xffffu), dot);
-      dot = fmaf(bf16_to_f32(a[m] >> 16), bf16_to_f32(b[m] >> 16), dot);
+    for (int s = 0; s < T::kK; ++s) {
+      if (s < kQReg) qf[s] = x[s];
+      else *reinterpret_cast<lds_u32x4*>(qmine + ((s - kQReg) * 64 + lane) * 16) = __builtin_bit_cast(u32x4, x[s]);
     }
+    frags_of_rows<D>(b, box, lane, dof);
+    frags_of_rows<D>(c, box, lane, x);
+#pragma unroll
+    for (int s = 0; s < T::kK; ++s) {
+      const u32x4 y = __builtin_bit_cast(u32x4, dof[s]), z = __builtin_bit_cast(u32x4, x[s]);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        dot = fmaf(bf16_to_f32(y[m] & 0xffffu), bf16_to_f32(z[m] & 0xffffu), dot);
+        dot = fmaf(bf16_to_f32(y[m] >> 16), bf16_to_f32(z[m] >> 16), dot);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
   dot = half_swap_sum(dot);
   // a row without keys, and a row past the last, has P = exp2(-inf) = 0
   float lse2 = INFINITY, nd = 0.f;
   if (real) {
-    const float l = p.lse[token * n_heads + qhead];
+    const int64_t at = (sp.q0 + r / group) * n_heads + (int64_t)head * group + r % group;
+    const float l = p.lse[at];
     lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
-    nd = (p.dlse != nullptr ? p.dlse[token * n_heads + qhead] : 0.f) - dot;
+    nd = (p.dlse != nullptr ? p.dlse[at] : 0.f) - dot;
   }
 
   const uint16_t* kbase = p.k + (int64_t)sp.k0 * p.ks + head * p.kh;
@@ -190,7 +204,6 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   float sum = 0.f, sum_r = 0.f;  // of dS, and of dS as rounded
   const float c = p.scale_log2;
 
-  lds_u8* const s0 = (lds_u8*)ring[0];
   if (n_steps > 0) load_step(0, s0);
   for (int u = 0; u < n_steps; ++u) {
     const lds_u8* cur = s0 + (u & 1) * kSlot;
@@ -256,24 +269,28 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
       }
     }
   }
+  // (the row's place again, from the lane's index: held through the walk it
+  // would cost the registers that the products need)
+  const int ln = lane_anew();
+  const int row = r0 + 32 * wave + (ln & 31);
+  const int64_t at = (sp.q0 + row / group) * n_heads + (int64_t)head * group + row % group;
   // dS of a row sums to dLSE: what its rounded values sum to beside that has
   // gone to the row's mean key, and -D is off by what the exact ones do
   sum = half_swap_sum(sum);
   sum_r = half_swap_sum(sum_r);
-  const float dl = real && p.dlse != nullptr && lse2 != INFINITY ? p.dlse[token * n_heads + qhead] : 0.f;
-  if (hi == 0) {
+  const float dl = row < rows && p.dlse != nullptr && lse2 != INFINITY ? p.dlse[at] : 0.f;
+  if (ln < 32) {
     float* rec = p.rec + (((int64_t)head * p.q_slots + slot) * 2 + (wave >> 1)) * kRecFloats;
-    rec[32 * (wave & 1) + li] = lse2;
-    rec[64 + 32 * (wave & 1) + li] = nd - (sum - dl);
+    rec[32 * (wave & 1) + ln] = lse2;
+    rec[64 + 32 * (wave & 1) + ln] = nd - (sum - dl);
   }
 #pragma unroll
   for (int t = 0; t < T::kT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(dl - sum_r, mean[t][e], acc[t][e]);
   __syncthreads();  // every wave is done with the ring
-  uint16_t* const mine = p.dq + (token * n_heads + qhead) * D;
-  const uint64_t bits = reinterpret_cast<uintptr_t>(mine);
-  store_rows<D>(acc, p.scale, s0 + wave * 32 * T::kPitch, lane, [&](int rr) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(p.dq + at * D);
+  store_rows<D>(acc, p.scale, s0 + wave * 32 * T::kPitch, ln, [&](int rr) {
     const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)bits, rr);
     const uint32_t up = (uint32_t)__shfl((int)(uint32_t)(bits >> 32), rr);
     return r0 + 32 * wave + rr < rows
@@ -340,7 +357,6 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   // (exact: x < 64 + group, and x group < 2^32).
   int t0 = (int)((int64_t)64 * u0 / group), rem = (int)((int64_t)64 * u0 - (int64_t)t0 * group);
   const int t_step = 64 / group, r_step = 64 - t_step * group;
-  const uint32_t per_group = 0xffffffffu / (uint32_t)group + 1;  // 0 for a group of one
   auto load_step = [&](int u, lds_u8* dst) {
     const int lane = lane_anew();
     const char* qb = reinterpret_cast<const char*>(qhead + (int64_t)t0 * p.qs);
@@ -350,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
       const int seg = T::kSegs * wave + s;
       const int row = seg * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
       const uint32_t x = (uint32_t)(min(row, rows - 1 - 64 * u) + rem);
-      const uint32_t t = group == 1 ? x : __umulhi(x, per_group), g = x - t * (uint32_t)group;
+      const uint32_t t = group == 1 ? x : __umulhi(x, p.per_group), g = x - t * (uint32_t)group;
       const uint32_t ch = (uint32_t)((pos ^ swz_both<D>(row)) << 4);
       dma16(qb, t * (uint32_t)(2 * p.qs) + g * (uint32_t)(2 * p.qh) + ch, dst + seg * 1024);
       dma16(db, t * (uint32_t)(2 * p.dos) + g * (uint32_t)(2 * p.doh) + ch,
@@ -580,6 +596,7 @@ extern "C" int veda_packed_bwd(
   p.rec = static_cast<float*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + rec_bytes);
   p.n_split = (int32_t)n_split;
+  p.per_group = per_group_of((uint32_t)p.pk.group);
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);

@@ -41,40 +41,46 @@ __device__ __forceinline__ int32_t cu_at(const int32_t* cu, int i, int n_seq, in
   return i < 0 ? 0 : i > n_seq ? rows : min(max(cu[i], 0), rows);
 }
 
-// The sequence of slot `slot` (of rows with `mult` rows a packed row), by all
-// lanes of a wave at once: 64 candidates a round. Offsets that do not ascend
-// give some sequence, whose rows are within the tensors all the same.
-__device__ __forceinline__ int seq_of_slot(const int32_t* cu, int n_seq, int32_t rows, int mult,
-                                           int slot, int lane) {
-  int lo = 0, count = n_seq + 2;
-  while (count > 1) {
+// The span of slot `slot`, by all lanes of a wave at once, 64 candidates a round;
+// the last round's lanes hold the offsets of both sides, so the sequence's own
+// come from the lanes beside each other. of_keys: slots count tiles of keys, not
+// of query rows. Offsets that do not ascend give some sequence, whose rows are
+// within the tensors all the same.
+__device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int slot, int lane) {
+  const int32_t* cu = of_keys ? p.cu_k : p.cu_q;
+  const int32_t* other = of_keys ? p.cu_q : p.cu_k;
+  const int32_t rows = of_keys ? p.k_rows : p.q_rows, other_rows = of_keys ? p.q_rows : p.k_rows;
+  const int mult = of_keys ? 1 : p.group;
+  const int last = p.n_seq + 1;
+  int lo = 0, count = last + 1;
+  while (count > 64) {
     const int stride = (count + 63) >> 6;
-    const int i = lo + lane * stride;
-    const bool in = i < lo + count;
-    const int64_t at = ((int64_t)cu_at(cu, in ? i - 1 : lo - 1, n_seq, rows) * mult) / kRows + i;
-    const uint64_t below = __ballot(in && at <= slot);
-    const int hits = max((int)__builtin_popcountll(below), 1);
-    const int next = lo + (hits - 1) * stride;
+    const int i = min(lo + lane * stride, lo + count - 1);
+    const int64_t at = ((int64_t)cu_at(cu, i - 1, p.n_seq, rows) * mult) / kRows + i;
+    const uint64_t below = __ballot(lane * stride < count && at <= slot);
+    const int next = lo + (max((int)__builtin_popcountll(below), 1) - 1) * stride;
     count = min(stride, lo + count - next);
     lo = next;
   }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
-
-// The span of a slot; of_keys: slots count tiles of keys, not of query rows.
-__device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int slot, int lane) {
-  const int32_t* cu = of_keys ? p.cu_k : p.cu_q;
-  const int32_t rows = of_keys ? p.k_rows : p.q_rows;
-  const int mult = of_keys ? 1 : p.group;
-  const int i = seq_of_slot(cu, p.n_seq, rows, mult, slot, lane);
+  // lane: where sequence lo + lane begins, which is where the one before it ends
+  const int32_t mine = cu_at(cu, lo + lane - 1, p.n_seq, rows);
+  const int32_t its = cu_at(other, lo + lane - 1, p.n_seq, other_rows);
+  const int64_t at = ((int64_t)mine * mult) / kRows + lo + lane;
+  const uint64_t below = __ballot(lane < count && at <= slot);
+  const int hit = max((int)__builtin_popcountll(below), 1) - 1;
+  const int i = __builtin_amdgcn_readfirstlane(lo + hit);
+  const int32_t begin = __builtin_amdgcn_readlane(mine, hit);
+  const int32_t other_begin = __builtin_amdgcn_readlane(its, hit);
+  const int32_t end = hit < 63 ? __builtin_amdgcn_readlane(mine, hit + 1) : cu_at(cu, i, p.n_seq, rows);
+  const int32_t other_end =
+      hit < 63 ? __builtin_amdgcn_readlane(its, hit + 1) : cu_at(other, i, p.n_seq, other_rows);
   Span s;
-  s.q0 = cu_at(p.cu_q, i - 1, p.n_seq, p.q_rows);
-  s.nq = max(cu_at(p.cu_q, i, p.n_seq, p.q_rows) - s.q0, 0);
-  s.k0 = cu_at(p.cu_k, i - 1, p.n_seq, p.k_rows);
-  s.nk = max(cu_at(p.cu_k, i, p.n_seq, p.k_rows) - s.k0, 0);
-  const int32_t begin = of_keys ? s.k0 : s.q0;
+  s.q0 = of_keys ? other_begin : begin;
+  s.nq = max(of_keys ? other_end - other_begin : end - begin, 0);
+  s.k0 = of_keys ? begin : other_begin;
+  s.nk = max(of_keys ? end - begin : other_end - other_begin, 0);
   s.tile = slot - (int)(((int64_t)begin * mult) / kRows + i);
-  if (i == 0 || i == p.n_seq + 1) {  // rows of no sequence: no key, no query
+  if (i == 0 || i == last) {  // rows of no sequence: no key, no query
     if (of_keys) s.nq = 0;
     else s.nk = 0;
   }
@@ -152,6 +158,58 @@ __device__ __forceinline__ f32x16 zero16() {
 #pragma unroll
   for (int e = 0; e < 16; ++e) z[e] = 0.f;
   return z;
+}
+
+// A wave's 32 packed rows r0 .. of a tensor [rows, heads, D] (`x` at the span's
+// first row and the group's first head), zeros past `rows`: read as whole rows
+// into registers, kSegRows a load. A fragment read straight from memory takes 32
+// bytes of each of 32 rows, so a line comes in four times over once the rows of
+// the waves beside it have pushed it out of L1.
+template <int D>
+struct RowLoads {
+  u32x4 x[32 / Tile<D>::kSegRows];
+};
+
+template <int D>
+__device__ __forceinline__ RowLoads<D> load_rows(const uint16_t* x, int64_t stride_s, int64_t stride_h,
+                                                 int group, uint32_t per_group, int r0, int rows,
+                                                 int lane) {
+  using T = Tile<D>;
+  RowLoads<D> res;
+  const int t0 = r0 / group, rem = r0 - t0 * group;  // wave-uniform
+#pragma unroll
+  for (int i = 0; i < 32 / T::kSegRows; ++i) {
+    const int rr = i * T::kSegRows + lane / T::kChunks;
+    const uint32_t y = (uint32_t)(rr + rem);
+    const uint32_t t = group == 1 ? y : __umulhi(y, per_group), g = y - t * (uint32_t)group;
+    res.x[i] = u32x4{0, 0, 0, 0};
+    if (r0 + rr < rows)
+      res.x[i] = ld16(x + (t0 + (int64_t)t) * stride_s + (int64_t)g * stride_h + 8 * (lane % T::kChunks));
+  }
+  return res;
+}
+
+// 2^32 / group for divisions of less than 2^32 / group by it (0 for one).
+__host__ __device__ inline uint32_t per_group_of(uint32_t group) { return 0xffffffffu / group + 1; }
+
+// Those rows as B operand fragments (lane: row lane % 32, chunk 2 s + lane / 32),
+// by way of the wave's own 32 rows of LDS.
+template <int D>
+__device__ __forceinline__ void frags_of_rows(const RowLoads<D>& r, lds_u8* box, int lane,
+                                              bf16x8 (&f)[Tile<D>::kK]) {
+  using T = Tile<D>;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  const int li = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < 32 / T::kSegRows; ++i) {
+    const int rr = i * T::kSegRows + lane / T::kChunks, pos = lane % T::kChunks;
+    *reinterpret_cast<lds_u32x4*>(box + rr * T::kPitch + ((pos ^ swz_row<D>(rr)) << 4)) = r.x[i];
+  }
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < T::kK; ++s)
+    f[s] = lds_frag(box + li * T::kPitch + (((2 * s + hi) ^ swz_row<D>(li)) << 4));
+  asm volatile("" ::: "memory");
 }
 
 inline bool rows16(const void* p, int64_t s, int64_t h) {
