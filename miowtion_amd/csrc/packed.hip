@@ -353,8 +353,10 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
 #pragma unroll
     for (int s = 0; s < T::kK; ++s) asm volatile("" : : "v"(w.qf[s]));
     sync();
+    if (n_steps > 1) {
 #pragma unroll
-    for (int s = 0; s < T::kSegs; ++s) issue(k1, s, lds0 + kSlot);
+      for (int s = 0; s < T::kSegs; ++s) issue(k1, s, lds0 + kSlot);
+    }
     stage<D, true, kNoSm, false>(s0, s0, f, c, sa, sb, pb, pa, w, NoHook{});
     stage<D, true, kNoSm, false>(s0 + kSub, s0, f, c, sb, sa, pa, pb, w, NoHook{});
     if (n_plain == 0) {
