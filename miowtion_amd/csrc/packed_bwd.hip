@@ -205,70 +205,94 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   const float c = p.scale_log2;
 
   if (n_steps > 0) load_step(0, s0);
-  for (int u = 0; u < n_steps; ++u) {
-    const lds_u8* cur = s0 + (u & 1) * kSlot;
-    VEDA_WAIT_VM(0);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (u + 1 < n_steps) load_step(u + 1, s0 + ((u + 1) & 1) * kSlot);
+  // MASK: some row does not see some key of the steps
+  auto walk = [&](auto mask, int from, int to) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask)::value;
 #pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
-      const int ln = lane_anew();
-      const uint32_t ra = row_offset<D>(ln), ta = tr_offset<D>(ln, 0, 0, swz_both<D>);
-      const lds_u8* ks = cur + sub * 32 * T::kPitch;
-      const lds_u8* vs = ks + T::kBytes;
-      f32x16 st = zero16(), dp;
+    for (int u = from; u < to; ++u) {
+      const lds_u8* cur = s0 + (u & 1) * kSlot;
+      VEDA_WAIT_VM(0);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (u + 1 < n_steps) load_step(u + 1, s0 + ((u + 1) & 1) * kSlot);
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) {
+        const int ln = lane_anew();
+        const uint32_t ra = row_offset<D>(ln), ta = tr_offset<D>(ln, 0, 0, swz_both<D>);
+        const lds_u8* ks = cur + sub * 32 * T::kPitch;
+        const lds_u8* vs = ks + T::kBytes;
+        f32x16 st = zero16(), dp;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dp[e] = nd;
-      bf16x8 ka[T::kK], va[T::kK];
-      ka[0] = lds_frag(ks + ra);
-      va[0] = lds_frag(vs + ra);
+        for (int e = 0; e < 16; ++e) dp[e] = nd;
+        bf16x8 ka[T::kK], va[T::kK];
+        ka[0] = lds_frag(ks + ra);
+        ka[1] = lds_frag(ks + (ra ^ 32));
 #pragma unroll
-      for (int s = 0; s < T::kK; ++s) {
-        if (s + 1 < T::kK) {
-          ka[s + 1] = lds_frag(ks + (ra ^ (32 * (s + 1))));
-          va[s + 1] = lds_frag(vs + (ra ^ (32 * (s + 1))));
+        for (int s = 0; s < T::kK; ++s) {
+          if (s + 2 < T::kK) ka[s + 2] = lds_frag(ks + (ra ^ (32 * (s + 2))));
+          else va[s + 2 - T::kK] = lds_frag(vs + (ra ^ (32 * (s + 2 - T::kK))));
+          st = mfma32(ka[s], s < kQReg ? qf[s % kQReg] : lds_frag(qmine + ((s - kQReg) * 64 + ln) * 16), st);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        st = mfma32(ka[s], s < kQReg ? qf[s % kQReg] : lds_frag(qmine + ((s - kQReg) * 64 + ln) * 16), st);
-        dp = mfma32(va[s], dof[s], dp);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const int lim = u >= n_plain ? limit - 64 * u - 32 * sub - 4 * hi : 32;
-      u32x4 pb[2], db[2];
+        // dP - D, and the probabilities under its products
+        const int lim = limit - 64 * u - 32 * sub - 4 * hi;
+        auto sees = [&](int e) { return !MASK || 8 * (e >> 2) + (e & 3) < lim; };
+        constexpr int kPer = 16 / T::kK;
+        float pr[16];
+        u32x4 pb[2], db[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float pr[2], ds[2];
+        for (int s = 0; s < T::kK; ++s) {
+          if (s + 2 < T::kK) va[s + 2] = lds_frag(vs + (ra ^ (32 * (s + 2))));
+          dp = mfma32(va[s], dof[s], dp);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int e = 2 * j + m;
-          const bool see = 8 * (e >> 2) + (e & 3) < lim;
-          pr[m] = __builtin_amdgcn_exp2f(fmaf(st[e], c, -lse2));
-          ds[m] = see ? pr[m] * dp[e] : 0.f;
-          pr[m] = see ? pr[m] : 0.f;
+          for (int m = 0; m < kPer; ++m) {
+            const int e = kPer * s + m;
+            const float x = __builtin_amdgcn_exp2f(fmaf(st[e], c, -lse2));
+            pr[e] = sees(e) ? x : 0.f;
+            if (e & 1) pb[e >> 3][(e >> 1) & 3] = pack_bf16x2(pr[e - 1], pr[e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        pb[j >> 2][j & 3] = pack_bf16x2(pr[0], pr[1]);
-        const uint32_t y = pack_bf16x2(ds[0], ds[1]);
-        db[j >> 2][j & 3] = y;
-        sum += ds[0] + ds[1];
-        sum_r = add_pair(y, sum_r);
-      }
-      auto tr = [&](int i) {  // keys 16 (i / kT), column block i % kT
-        const lds_u8* a = ks + (i / T::kT) * 16 * T::kPitch;
-        const uint32_t at = ta ^ (64 * (i % T::kT));
-        return join_tr(a + at, a + (at ^ (8 * T::kPitch + 32)));
-      };
-      bf16x8 kt[2 * T::kT];
-      kt[0] = tr(0);
-      __builtin_amdgcn_sched_barrier(0);
+        auto tr = [&](int i) {  // keys 16 (i / kT), column block i % kT
+          const lds_u8* a = ks + (i / T::kT) * 16 * T::kPitch;
+          const uint32_t at = ta ^ (64 * (i % T::kT));
+          return join_tr(a + at, a + (at ^ (8 * T::kPitch + 32)));
+        };
+        // dS of two keys (pair j of the lane's eight)
+        auto pair = [&](int j) {
+          float ds[2];
 #pragma unroll
-      for (int i = 0; i < 2 * T::kT; ++i) {
-        if (i + 1 < 2 * T::kT) kt[i + 1] = tr(i + 1);
-        acc[i % T::kT] = mfma32(kt[i], as_bf16x8(db[i / T::kT]), acc[i % T::kT]);
-        mean[i % T::kT] = mfma32(kt[i], as_bf16x8(pb[i / T::kT]), mean[i % T::kT]);
+          for (int m = 0; m < 2; ++m) {
+            const int e = 2 * j + m;
+            ds[m] = sees(e) ? pr[e] * dp[e] : 0.f;
+          }
+          const uint32_t y = pack_bf16x2(ds[0], ds[1]);
+          db[j >> 2][j & 3] = y;
+          sum += ds[0] + ds[1];
+          sum_r = add_pair(y, sum_r);
+        };
+        // dS K and P K, the second 16 keys' dS under the first's products
+        bf16x8 kt[2 * T::kT];
+        kt[0] = tr(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pair(j);
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2 * T::kT; ++i) {
+          if (i + 1 < 2 * T::kT) kt[i + 1] = tr(i + 1);
+          acc[i % T::kT] = mfma32(kt[i], as_bf16x8(db[i / T::kT]), acc[i % T::kT]);
+          if (i < T::kT) {
+#pragma unroll
+            for (int j = 0; j < 4 / T::kT; ++j) pair(4 + i * (4 / T::kT) + j);
+          }
+          mean[i % T::kT] = mfma32(kt[i], as_bf16x8(pb[i / T::kT]), mean[i % T::kT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
-  }
+  };
+  walk(std::false_type{}, 0, min(n_plain, n_steps));
+  walk(std::true_type{}, min(n_plain, n_steps), n_steps);
   // (the row's place again, from the lane's index: held through the walk it
   // would cost the registers that the products need)
   const int ln = lane_anew();
