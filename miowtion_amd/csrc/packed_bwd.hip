@@ -344,10 +344,13 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
     const int64_t i = (int64_t)j - (sp.nk - sp.nq);
     return p.pk.causal ? (int)min(max(i * group, (int64_t)0), (int64_t)rows) : 0;
   };
-  const int first_step = first(j0) >> 6, end_step = (rows + 63) >> 6;  // the steps that see the tile, and this split's
-  const int n_all = max(end_step - first_step, 0);
-  const int u0 = first_step + (int)((int64_t)n_all * split / p.n_split);
-  const int u1 = first_step + (int)((int64_t)n_all * (split + 1) / p.n_split);
+  // The steps that see the tile, from the last row down, every n_split-th of
+  // them here: the workgroups of a head then walk the same rows at about the same
+  // time, and find them in L2 (from each tile's own first row up, they did not).
+  const int first_step = first(j0) >> 6, end_step = (rows + 63) >> 6;
+  const int top = end_step - 1 - split;
+  const int n_steps = top >= first_step ? (top - first_step) / p.n_split + 1 : 0;
+  auto step = [&](int k) { return top - k * p.n_split; };
   const int w0 = j0 + 32 * wave;                       // this wave's keys
   const int key = min(w0 + li, sp.nk - 1);
   const int mine = first(key);
@@ -379,8 +382,12 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   // The steps' rows are loaded in turn: t0, rem are the next step's first token
   // and head. Row x from there is token x / group by a product with 2^32 / group
   // (exact: x < 64 + group, and x group < 2^32).
-  int t0 = (int)((int64_t)64 * u0 / group), rem = (int)((int64_t)64 * u0 - (int64_t)t0 * group);
-  const int t_step = 64 / group, r_step = 64 - t_step * group;
+  int t0 = 0, rem = 0;
+  if (n_steps > 0) {
+    t0 = (int)((int64_t)64 * top / group);
+    rem = (int)((int64_t)64 * top - (int64_t)t0 * group);
+  }
+  const int t_step = 64 * p.n_split / group, r_step = 64 * p.n_split - t_step * group;
   auto load_step = [&](int u, lds_u8* dst) {
     const int lane = lane_anew();
     const char* qb = reinterpret_cast<const char*>(qhead + (int64_t)t0 * p.qs);
@@ -396,11 +403,11 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
       dma16(db, t * (uint32_t)(2 * p.dos) + g * (uint32_t)(2 * p.doh) + ch,
             dst + T::kBytes + seg * 1024);
     }
-    t0 += t_step;
-    rem += r_step;
-    if (rem >= group) {
-      rem -= group;
-      ++t0;
+    t0 -= t_step;
+    rem -= r_step;
+    if (rem < 0) {
+      rem += group;
+      --t0;
     }
     if (wave == 0)
       dma16(reinterpret_cast<const char*>(recs + (int64_t)u * kRecFloats), (uint32_t)((lane & 31) * 16),
@@ -487,15 +494,16 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   };
 
   lds_u8* const s0 = (lds_u8*)ring[0];
-  if (u0 < u1) load_step(u0, s0 + (u0 & 1) * kSlot);
+  if (n_steps > 0) load_step(top, s0);
   auto walk = [&](auto mask, int from, int to) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int u = from; u < to; ++u) {
-      const lds_u8* cur = s0 + (u & 1) * kSlot;
+    for (int k = from; k < to; ++k) {
+      const lds_u8* cur = s0 + (k & 1) * kSlot;
+      const int u = step(k);
       VEDA_WAIT_VM(0);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (u + 1 < u1) load_step(u + 1, s0 + ((u + 1) & 1) * kSlot);
+      if (k + 1 < n_steps) load_step(step(k + 1), s0 + ((k + 1) & 1) * kSlot);
       if (!live) continue;
       if (decltype(mask)::value) {
 #pragma unroll 1
@@ -507,9 +515,11 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
       }
     }
   };
-  const int um = max(min((full_from + 63) >> 6, u1), u0);
-  walk(std::true_type{}, u0, um);
-  walk(std::false_type{}, um, u1);
+  // steps from full_step on see all of the wave's keys
+  const int full_step = (full_from + 63) >> 6;
+  const int n_plain = top >= full_step ? min((top - full_step) / p.n_split + 1, n_steps) : 0;
+  walk(std::false_type{}, 0, n_plain);
+  walk(std::true_type{}, n_plain, n_steps);
 
   __syncthreads();  // every wave is done with the ring
   const int64_t ld = (int64_t)p.pk.n_kv * D;
