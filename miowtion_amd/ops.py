@@ -95,9 +95,9 @@ class _Op:
         if kwargs or not _ordinary(args, self._kinds):
             return self._op(*args, **kwargs)
         out = self._fn(*args)
-        for i in self._mutated:
-            if args[i] is not None:
-                torch.autograd.graph.increment_version(args[i])
+        if self._mutated:
+            torch.autograd.graph.increment_version(
+                [args[i] for i in self._mutated if args[i] is not None])
         return out
 
     def __getattr__(self, name):

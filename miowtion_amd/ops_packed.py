@@ -125,8 +125,8 @@ def _splits(k_rows: int, kv_heads: int) -> int:
     keys have most of the rows, so tiles that fill the GPU once end unevenly; a
     split's sums cost 16 bytes of traffic for each value of dk. Forward and
     backward with 1, 2, 3, 4 and 8 splits: 64 tiles x 4 key heads (8,192 tokens, 28
-    heads) 3,404, 2,494, 2,246, 2,281 and 2,247 us; 48 x 8 (6,039 tokens of twelve
-    prompts, 32 heads) 407, 379, 378, 384 and 469 us."""
+    heads) 3,000, 2,368, 2,214, 2,222 and 2,201 us; 48 x 8 (6,039 tokens of twelve
+    prompts, 32 heads) 374, 359, 363, 369 and 455 us."""
     return min(max(-(-768 // (max(-(-k_rows // TILE), 1) * kv_heads)), 1), 16)
 
 

@@ -71,6 +71,8 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, dout, dlse):
         q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
         dout = torch.zeros_like(out) if dout is None else dout.contiguous()
+        if dout.data_ptr() % 16:  # a view whose rows begin off a 16-byte boundary
+            dout = dout.clone()
         dq, dk, dv = ops_packed.packed_bwd(q, k, v, out, dout, lse,
                                            None if dlse is None else dlse.contiguous(), cu_q, cu_k,
                                            ctx.causal, ctx.scale)

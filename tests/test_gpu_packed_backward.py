@@ -121,6 +121,21 @@ def test_expanded_inputs_and_gradients():
         pr.check(t.grad, ref, name)
 
 
+def test_output_gradients_in_any_place():
+    """A transposed gradient, and one that begins off a 16-byte boundary."""
+    lens = [70, 3]
+    q, k, v = _inputs(lens, lens, 4, 2, 64)
+    cu = pr.offsets(lens)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    want = _grads(q, k, v, cu, None, True, dout)
+    turned = dout.transpose(0, 1).contiguous().transpose(0, 1)
+    moved = torch.empty(dout.numel() + 8, dtype=dout.dtype, device='cuda')[1:1 + dout.numel()].view(dout.shape)
+    moved.copy_(dout)
+    for d in (turned, moved):
+        for a, b in zip(_grads(q, k, v, cu, None, True, d), want):
+            assert torch.equal(a, b)
+
+
 def _half_sums(q, k, v, lens):
     """Per pair of query heads the gradient's magnitude, summed."""
     res = None
