@@ -45,7 +45,7 @@ __device__ __forceinline__ int32_t cu_at(const int32_t* cu, int i, int n_seq, in
 // the last round's lanes hold the offsets of both sides, so the sequence's own
 // come from the lanes beside each other. of_keys: slots count tiles of keys, not
 // of query rows. Offsets that do not ascend give some sequence, whose rows are
-// within the tensors all the same.
+// within the tensors all the same, or no tile.
 __device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int slot, int lane) {
   const int32_t* cu = of_keys ? p.cu_k : p.cu_q;
   const int32_t* other = of_keys ? p.cu_q : p.cu_k;
@@ -80,6 +80,7 @@ __device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int
   s.k0 = of_keys ? begin : other_begin;
   s.nk = max(of_keys ? end - begin : other_end - other_begin, 0);
   s.tile = slot - (int)(((int64_t)begin * mult) / kRows + i);
+  if (s.tile < 0) s.tile = 1 << 23;  // offsets do not ascend: a tile past every row
   if (i == 0 || i == last) {  // rows of no sequence: no key, no query
     if (of_keys) s.nq = 0;
     else s.nk = 0;

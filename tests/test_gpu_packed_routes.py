@@ -143,3 +143,52 @@ def test_long_sequences(d):
     ref = pr.attend(q, k, v, lens, lens, dout=dout)
     for name, x in zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *torch.autograd.grad(out, ts, dout))):
         pr.check(x, ref, name)
+
+
+MANY = [
+    # sequences, longest, heads, kv, d, causal, chunk: several workgroups to each
+    # place on the device, their walks of very different lengths
+    (40, 700, 16, 4, 128, True, False),
+    (40, 700, 16, 4, 64, False, False),
+    (120, 300, 14, 2, 64, True, False),
+    (9, 1500, 24, 8, 64, True, True),
+    (24, 1500, 24, 8, 64, True, True),
+    (126, 200, 20, 20, 64, True, True),
+    (127, 200, 20, 20, 64, True, False),
+]
+
+
+@pytest.mark.parametrize('case', MANY, ids=lambda c: '-'.join(map(str, c)))
+def test_many_tiles_of_different_lengths(case):
+    n, longest, heads, kv, d, causal, chunk = case
+    g = torch.Generator().manual_seed(n)
+    lens_k = torch.randint(0, longest, (n,), generator=g).tolist()
+    lens_q = [min(m, int(torch.randint(0, 500, (1,), generator=g))) for m in lens_k] if chunk else lens_k
+    lens_k[n // 2] = lens_q[n // 2] = 0
+    print(f'{case}: {sum(lens_q) * heads // 128} query tiles', flush=True)
+    q, k, v = _inputs(lens_q, lens_k, heads, kv, d, seed=n, pad_q=130, pad_k=3)
+    dout = torch.randn(q.shape, generator=g).to(BF16).cuda()
+    ts = [t.requires_grad_(True) for t in (q, k, v)]
+    out, lse = kernels.packed_attention(*ts, pr.offsets(lens_q), pr.offsets(lens_k), causal=causal,
+                                        return_lse=True)
+    ref = pr.attend(q, k, v, lens_q, lens_k, causal, dout=dout)
+    pr.check(lse.detach(), ref, 'lse')
+    for name, x in zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *torch.autograd.grad(out, ts, dout))):
+        pr.check(x, ref, name)
+
+
+def test_offsets_out_of_order():
+    """Offsets that do not ascend name no sequences: what they give is not said,
+    but the calls end, and their inputs stay."""
+    g = torch.Generator().manual_seed(3)
+    for n in (2, 5, 61, 62, 63, 200):
+        heads, kv, d = 6, 2, 64
+        cu_q, cu_k = (torch.randint(-50, 1000, (n + 1,), generator=g).int().cuda() for _ in range(2))
+        q, k, v = (torch.full((rows, h, d), 3.0, dtype=BF16, device='cuda')
+                   for rows, h in ((700, heads), (600, kv), (600, kv)))
+        out, lse = kernels.packed_attention(q, k, v, cu_q, cu_k, return_lse=True)
+        grads = ops_packed.packed_bwd(q, k, v, out, q, lse, None, cu_q, cu_k, True, d ** -0.5)
+        torch.cuda.synchronize()
+        print(f'{n} sequences', flush=True)
+        assert all((x == 3.0).all() for x in (q, k, v))
+        assert [x.shape for x in grads] == [q.shape, k.shape, v.shape]
