@@ -244,8 +244,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
   const int item = (int)(blockIdx.x / p.pk.n_kv);
-  const int slot = p.n_slots - 1 - item / p.n_split, split = item % p.n_split;
-  const Span sp = span_of_slot(p.pk, false, slot, lane);
+  const int split = item % p.n_split;
+  const Span sp = span_of(p.pk, false, item / p.n_split, p.n_slots, lane);
   const int rows = sp.nq * p.pk.group;
   const int r0 = sp.tile * kRows;
   if (r0 >= rows) return;
@@ -514,7 +514,8 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
   if (q_rows == 0) return VEDA_OK;
   FwdArgs p{};
   p.pk = Packing{cu_q, cu_k, (int32_t)n_seq, (int32_t)q_rows, (int32_t)k_rows, (int32_t)n_kv_heads,
-                 (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0};
+                 (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0,
+                 ranked(n_seq, q_rows * n_heads / kRows * n_split), 0};
   p.q = static_cast<const uint16_t*>(q);
   p.k = static_cast<const uint16_t*>(k);
   p.v = static_cast<const uint16_t*>(v);

@@ -126,8 +126,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
-  const int slot = p.q_slots - 1 - (int)(blockIdx.x / p.pk.n_kv);
-  const Span sp = span_of_slot(p.pk, false, slot, lane);
+  const Span sp = span_of(p.pk, false, (int)(blockIdx.x / p.pk.n_kv), p.q_slots, lane);
   const int group = p.pk.group, rows = sp.nq * group;
   const int r0 = sp.tile * kRows;
   if (r0 >= rows) return;
@@ -304,6 +303,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   sum_r = half_swap_sum(sum_r);
   const float dl = row < rows && p.dlse != nullptr && lse2 != INFINITY ? p.dlse[at] : 0.f;
   if (ln < 32) {
+    const int slot = first_q_slot(p.pk, sp) + sp.tile;
     float* rec = p.rec + (((int64_t)head * p.q_slots + slot) * 2 + (wave >> 1)) * kRecFloats;
     rec[32 * (wave & 1) + ln] = lse2;
     rec[64 + 32 * (wave & 1) + ln] = nd - (sum - dl);
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
   const int item = (int)(blockIdx.x / p.pk.n_kv);
-  const int slot = item / p.n_split, split = item % p.n_split;  // causal: the first keys have the most rows
-  const Span sp = span_of_slot(p.pk, true, slot, lane);
+  const int split = item % p.n_split;
+  const Span sp = span_of(p.pk, true, item / p.n_split, p.k_slots, lane);
   const int j0 = sp.tile * kRows;
   if (j0 >= sp.nk) return;
   const int group = p.pk.group, rows = sp.nq * group;
@@ -373,9 +373,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   for (int t = 0; t < T::kT; ++t) acc_v[t] = acc_k[t] = zero16();
   const float c = p.scale_log2;
   // records of the sequence's rows: its first query slot's on
-  const int q_slot0 = (int)(((int64_t)sp.q0 * group) / kRows) +
-                      (slot - sp.tile - (int)(sp.k0 / kRows));
-  const float* recs = p.rec + ((int64_t)head * p.q_slots + q_slot0) * 2 * kRecFloats;
+  const float* recs = p.rec + ((int64_t)head * p.q_slots + first_q_slot(p.pk, sp)) * 2 * kRecFloats;
   const uint16_t* qhead = p.q + (int64_t)sp.q0 * p.qs + (int64_t)head * group * p.qh;
   const uint16_t* dhead = p.dout + (int64_t)sp.q0 * p.dos + (int64_t)head * group * p.doh;
 
@@ -597,7 +595,9 @@ extern "C" int veda_packed_bwd(
     VEDA_REQUIRE(s >= 0 && s < (1 << 24), "packed_bwd: stride negative or too large");
   BwdArgs p{};
   p.pk = Packing{cu_q, cu_k, (int32_t)n_seq, (int32_t)q_rows, (int32_t)k_rows, (int32_t)n_kv_heads,
-                 (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0};
+                 (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0,
+                 ranked(n_seq, q_rows * n_heads / kRows),
+                 ranked(n_seq, k_rows * n_kv_heads / kRows * n_split)};
   VEDA_REQUIRE(p.pk.group <= 65000, "packed_bwd: at most 65000 query heads to a key head");
   VEDA_REQUIRE(p.pk.group <= 64 || (q_stride_h * p.pk.group < (1 << 30) &&
                                     do_stride_h * p.pk.group < (1 << 30)),

@@ -30,15 +30,27 @@ struct Packing {
   int32_t q_rows, k_rows;  // rows of q and of k, v
   int32_t n_kv, group;     // key heads; query heads of each
   int32_t causal;
+  int32_t ranked_q, ranked_k;  // tiles of query rows, of keys, by their sequences' length
 };
 
-// A tile's place: its sequence's queries and keys, and the tile's index in it.
+// A tile's place: its sequence's queries and keys, the tile's index in it, and the
+// sequence's in the list.
 struct Span {
-  int32_t q0, nq, k0, nk, tile;
+  int32_t q0, nq, k0, nk, tile, seq;
 };
 
+// A tile past every row, for workgroups that have none (its first row is 2^30).
+constexpr int32_t kNoTile = 1 << 23;
+
+// The first slot of query tiles of a span's sequence.
+__device__ __forceinline__ int first_q_slot(const Packing& p, const Span& s) {
+  return (int)(((int64_t)s.q0 * p.group) / kRows) + s.seq;
+}
+
+// Read without a branch, so that several are under way at once.
 __device__ __forceinline__ int32_t cu_at(const int32_t* cu, int i, int n_seq, int32_t rows) {
-  return i < 0 ? 0 : i > n_seq ? rows : min(max(cu[i], 0), rows);
+  const int32_t at = cu[min(max(i, 0), n_seq)];
+  return i < 0 ? 0 : i > n_seq ? rows : min(max(at, 0), rows);
 }
 
 // The span of slot `slot`, by all lanes of a wave at once, 64 candidates a round;
@@ -80,12 +92,115 @@ __device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int
   s.k0 = of_keys ? begin : other_begin;
   s.nk = max(of_keys ? end - begin : other_end - other_begin, 0);
   s.tile = slot - (int)(((int64_t)begin * mult) / kRows + i);
-  if (s.tile < 0) s.tile = 1 << 23;  // offsets do not ascend: a tile past every row
+  if (s.tile < 0) s.tile = kNoTile;  // offsets do not ascend
+  s.seq = i;
   if (i == 0 || i == last) {  // rows of no sequence: no key, no query
     if (of_keys) s.nq = 0;
     else s.nk = 0;
   }
   return s;
+}
+
+// The tile at place `rank` when the sequences are taken from the longest walk to
+// the shortest, for a long tile that starts late ends a launch alone: 30 prompts of
+// 20 to 1,500, 1,380 workgroups, took 73 us in the order given, 68 in this (42 and
+// 34 units of a step by list scheduling on 512 places); training on 20, 541 and
+// 515 us. Taking the tiles themselves in the order of their work mixes the
+// sequences, whose tiles then share no keys in the L2: 32 prompts of 512 took 79 us
+// so, 68 by sequence.
+//
+// By all lanes of a wave, two sequences each (the two of no sequence among them).
+// The place's level (walks of as many steps of 64) is found by bisection, its
+// sequence within the level by a prefix sum. Within a level a sequence's tiles begin
+// an eighth further on than the one's before: workgroups go round the XCDs and
+// their shader engines, and where sequences of one length have as many tiles as the
+// round, one engine would get the longest tile of each (the 32 prompts: 73 us).
+// Fewer tiles than 600 are resident nearly at once, in any order.
+constexpr int kRankedSeqs = 126;
+constexpr int64_t kRankedTiles = 600;
+
+// Each lane's sum (or maximum, of none below 0) of its own and all lanes' before
+// it: rows of 16 lanes in four steps, then over the rows' last lanes.
+template <bool MAX>
+__device__ __forceinline__ int lanes_upto(int x) {
+  auto put = [&](int y) { x = MAX ? max(x, y) : x + y; };
+  put(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr:1
+  put(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  put(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  put(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  put(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  put(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return x;
+}
+
+__device__ __forceinline__ Span span_of_rank(const Packing& p, bool of_keys, int rank, int lane) {
+  const int last = p.n_seq + 1;
+  int32_t q0[2], nq[2], k0[2], nk[2], tiles[2], steps[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = lane + 64 * h;
+    q0[h] = cu_at(p.cu_q, i - 1, p.n_seq, p.q_rows);
+    k0[h] = cu_at(p.cu_k, i - 1, p.n_seq, p.k_rows);
+    const int32_t q1 = cu_at(p.cu_q, i, p.n_seq, p.q_rows), k1 = cu_at(p.cu_k, i, p.n_seq, p.k_rows);
+    nq[h] = i > last ? 0 : max(q1 - q0[h], 0);
+    nk[h] = i > last ? 0 : max(k1 - k0[h], 0);
+    const uint32_t rows = (uint32_t)(nq[h] * p.group);  // < 2^31
+    tiles[h] = (int)(((of_keys ? (uint32_t)nk[h] : rows) + kRows - 1) / kRows);
+    if (i == 0 || i == last) {  // rows of no sequence: no key, no query
+      if (of_keys) nq[h] = 0;
+      else nk[h] = 0;
+    }
+    steps[h] = (int)(((of_keys ? (uint32_t)(nq[h] * p.group) : (uint32_t)nk[h]) + 63u) >> 6);
+  }
+  // tiles of walks of `level` steps or more
+  auto total = [&](int level) {
+    const int n = (steps[0] >= level ? tiles[0] : 0) + (steps[1] >= level ? tiles[1] : 0);
+    return __builtin_amdgcn_readlane(lanes_upto<false>(n), 63);
+  };
+  Span s{0, 0, 0, 0, kNoTile, 0};
+  if (rank >= total(0)) return s;
+  int lo = 0, hi = __builtin_amdgcn_readlane(lanes_upto<true>(max(steps[0], steps[1])), 63) + 1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (total(mid) > rank) lo = mid;
+    else hi = mid;
+  }
+  int left = rank - total(lo + 1);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int upto = lanes_upto<false>(steps[h] == lo ? tiles[h] : 0);
+    const int at = (int)__builtin_popcountll(__ballot(upto <= left));
+    if (at < 64) {
+      const int n = __builtin_amdgcn_readlane(tiles[h], at);
+      int in = left - (__builtin_amdgcn_readlane(upto, at) - n);
+      s.q0 = __builtin_amdgcn_readlane(q0[h], at);
+      s.nq = __builtin_amdgcn_readlane(nq[h], at);
+      s.k0 = __builtin_amdgcn_readlane(k0[h], at);
+      s.nk = __builtin_amdgcn_readlane(nk[h], at);
+      s.seq = __builtin_amdgcn_readfirstlane(at + 64 * h);
+      if (in < 0 || in >= n) return s;  // not where offsets ascend
+      const uint64_t level = __ballot(steps[h] == lo && lane < at);
+      in += (n * ((int)__builtin_popcountll(level) & 7)) >> 3;
+      if (in >= n) in -= n;
+      s.tile = of_keys ? in : n - 1 - in;
+      return s;
+    }
+    left -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return s;
+}
+
+// The tile of a workgroup; slots are taken from the last one where they count
+// query rows (causal: the last rows of a sequence see the most), from the first
+// where they count keys.
+__device__ __forceinline__ Span span_of(const Packing& p, bool of_keys, int item, int n_slots, int lane) {
+  if (of_keys ? p.ranked_k : p.ranked_q) return span_of_rank(p, of_keys, item, lane);
+  return span_of_slot(p, of_keys, of_keys ? item : n_slots - 1 - item, lane);
+}
+
+// Whether a launch over `tiles` workgroups takes the sequences by their length.
+inline int ranked(int64_t n_seq, int64_t tiles) {
+  return n_seq >= 2 && n_seq <= kRankedSeqs && tiles >= kRankedTiles && tiles < (1 << 20);
 }
 
 __host__ __device__ inline int64_t slots_of(int64_t rows, int64_t mult, int64_t n_seq) {

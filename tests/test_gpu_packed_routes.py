@@ -177,6 +177,19 @@ def test_many_tiles_of_different_lengths(case):
         pr.check(x, ref, name)
 
 
+@pytest.mark.parametrize('n,length', [(40, 130), (126, 64), (17, 300)])
+def test_many_sequences_of_one_length(n, length):
+    """Equal lengths: every tile of every sequence is met once."""
+    lens = [length] * n
+    q, k, v = _inputs(lens, lens, 32, 4, 64, seed=n)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(n)).to(BF16).cuda()
+    ts = [t.requires_grad_(True) for t in (q, k, v)]
+    out = kernels.packed_attention(*ts, pr.offsets(lens))
+    ref = pr.attend(q, k, v, lens, lens, dout=dout)
+    for name, x in zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *torch.autograd.grad(out, ts, dout))):
+        pr.check(x, ref, name)
+
+
 def test_offsets_out_of_order():
     """Offsets that do not ascend name no sequences: what they give is not said,
     but the calls end, and their inputs stay."""
