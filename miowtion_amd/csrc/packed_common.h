@@ -115,9 +115,11 @@ __device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int
 // an eighth further on than the one's before: workgroups go round the XCDs and
 // their shader engines, and where sequences of one length have as many tiles as the
 // round, one engine would get the longest tile of each (the 32 prompts: 73 us).
-// Fewer tiles than 600 are resident nearly at once, in any order.
+// Launches that are resident at once gain too: a CU's second workgroup is then a
+// short one (training on 20, keys not split: 519 and 486 us). Up to one to a CU, the
+// order is all the same.
 constexpr int kRankedSeqs = 126;
-constexpr int64_t kRankedTiles = 600;
+constexpr int64_t kRankedTiles = 256;
 
 // Each lane's sum (or maximum, of none below 0) of its own and all lanes' before
 // it: rows of 16 lanes in four steps, then over the rows' last lanes.

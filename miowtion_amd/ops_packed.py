@@ -119,15 +119,20 @@ def _(q, k, v, cu_q, cu_k, causal, scale, return_lse):
     return [out, q.new_empty(q.shape[:2], dtype=torch.float32)] if return_lse else [out]
 
 
-def _splits(k_rows: int, kv_heads: int) -> int:
-    """Workgroups that share the query rows of a key tile: 768 in all at least, one
-    and a half rounds of the 512 that are resident. Under a causal mask the first
-    keys have most of the rows, so tiles that fill the GPU once end unevenly; a
-    split's sums cost 16 bytes of traffic for each value of dk. Forward and
-    backward with 1, 2, 3, 4 and 8 splits: 64 tiles x 4 key heads (8,192 tokens, 28
-    heads) 3,000, 2,368, 2,214, 2,222 and 2,201 us; 48 x 8 (6,039 tokens of twelve
-    prompts, 32 heads) 374, 359, 363, 369 and 455 us."""
-    return min(max(-(-768 // (max(-(-k_rows // TILE), 1) * kv_heads)), 1), 16)
+def _splits(k_rows: int, kv_heads: int, walk: int = 1 << 14) -> int:
+    """Workgroups that share the query rows of a key tile: 512 in all at least, as
+    many as are resident, of four steps of 64 rows at least (`walk`: the rows of a
+    sequence for each key head, if half of the sequences hold all); half as many
+    again where walks are long, for under a causal mask the first keys have most of
+    the rows, and few sequences leave no others to fill in. A split's sums cost 16
+    bytes of traffic for each value of dk. Forward and backward in us with 1, 2, 3
+    and 4 splits: 8,192 tokens, 28 heads on 4 (256 tiles) 2,961, 2,298, 2,144, 2,152;
+    twelve prompts, 32 on 8 (378) 378, 335, 347, 365; 32 x 512, 16 on 4 (512) 299, 324,
+    340, 364; forty of up to 600, 32 on 8, head_dim 64 (764) 184, 204, 221, 242; 2,000
+    and fifteen of up to 100, 16 on 4 349, 248, 212, 197."""
+    tiles = max(-(-k_rows // TILE), 1) * kv_heads
+    want = 768 if walk >= 1 << 14 else 512
+    return max(min(-(-want // tiles), walk // 256, 16), 1)
 
 
 @_custom_op('veda::packed_bwd', mutates_args=())
@@ -149,7 +154,7 @@ def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Ten
             raise ValueError(f'{name} must be contiguous fp32 {[rows, heads]} on GPU {dev}')
     k_rows, kv, n_seq = k.shape[0], k.shape[1], cu_q.shape[0] - 1
     dq, dk, dv = q.new_empty(shape), k.new_empty(k.shape), k.new_empty(k.shape)
-    n_split = _splits(k_rows, kv)
+    n_split = _splits(k_rows, kv, rows * (heads // kv) // -(-max(n_seq, 1) // 2))
     work = q.new_empty(kv * (rows * (heads // kv) // TILE + n_seq + 2) * 256
                        + (2 * n_split * k_rows * kv * d if n_split > 1 else 0), dtype=_F32)
     _launch('veda_packed_bwd', dev, *tensors, lse.data_ptr(), _p(dlse), *sizes, causal, scale, n_split,
