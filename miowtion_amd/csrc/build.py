@@ -22,8 +22,9 @@ LIB = PKG / 'libveda_hip.so'
 BUILD_DIR = PKG / '_build'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
-# -packed-fp32-ops: hipcc must not emit packed fp32 arithmetic for this pool
-# (the host pass warns that it does not know the feature; harmless).
+# -packed-fp32-ops: hipcc must not emit packed fp32 arithmetic, some forms of which
+# have given wrong results (the host pass warns that it does not know the feature;
+# harmless).
 FLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}',
          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          f'-I{ROOT / "include"}']
