@@ -80,19 +80,17 @@ def _check_packed(q, k, v, cu_q, cu_k, scale):
 
 def _key_splits(q_rows: int, k_rows: int, n_seq: int, heads: int, kv_heads: int) -> int:
     """Workgroups that share the keys of 128 query rows: enough to fill the GPU
-    (512 are resident; a quarter more where the sequences are many times as long
-    as their queries, and end unevenly), of fifteen steps of 64 keys at least
-    where half of the sequences hold all of the keys. A split's sums cost 8 bytes
-    of traffic for each of its 32-bit values, so splits past that cost more than
-    they give. Times in us with 1, 2, 4, 8 and 16 splits: 2 x 16 queries of 16
-    heads over 52,768 keys 416, 220, 119, 70, 48; 512 of 32 over 8,192: 116, 82,
-    82, 94, 122; 4 x 512 of 32 (head_dim 64) over 21,388: 131, 117, 125, 147, 204;
-    whole prompts of 1,024, 1,000, 900 and 800 tokens, 8 heads: 26, 34, 43, 67, 129."""
+    (512 are resident), of fifteen steps of 64 keys at least where half of the
+    sequences hold all of the keys. A split's sums cost 8 bytes of traffic for each
+    of its 32-bit values, so splits past that cost more than they give. Times in us
+    with 1, 2, 4, 8 and 16 splits: 2 x 16 queries of 16 heads over 52,768 keys 419,
+    222, 119, 67, 43; 512 of 32 over 8,192: 115, 81, 79, 90, 113; 4 x 512 of 32
+    (head_dim 64) over 21,388: 107, 107, 119, 144, 202; whole prompts of 1,024, 1,000,
+    900 and 800 tokens, 8 heads: 25, 34, 44, 69, 129."""
     tiles = max(q_rows * heads // TILE, min(n_seq, q_rows) * kv_heads, 1)
-    want = 640 if 4 * q_rows <= k_rows else 512
-    if tiles >= want or n_seq == 0:
+    if tiles >= 512 or n_seq == 0:
         return 1
-    return max(min(-(-want // tiles), k_rows // -(-n_seq // 2) // 960, 32), 1)
+    return max(min(-(-512 // tiles), k_rows // -(-n_seq // 2) // 960, 32), 1)
 
 
 @_custom_op('veda::packed_fwd', mutates_args=())
