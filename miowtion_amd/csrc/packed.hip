@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
   const int head = blockIdx.x % p.pk.n_kv;
   const int item = (int)(blockIdx.x / p.pk.n_kv);
   const int split = item % p.n_split;
-  const Span sp = span_of(p.pk, false, item / p.n_split, p.n_slots, lane);
+  const Span sp = span_of(p.pk, false, item / p.n_split, p.n_slots, p.pk.n_kv * p.n_split, lane);
   const int rows = sp.nq * p.pk.group;
   const int r0 = sp.tile * kRows;
   if (r0 >= rows) return;

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
   const int head = blockIdx.x % p.pk.n_kv;
-  const Span sp = span_of(p.pk, false, (int)(blockIdx.x / p.pk.n_kv), p.q_slots, lane);
+  const Span sp = span_of(p.pk, false, (int)(blockIdx.x / p.pk.n_kv), p.q_slots, p.pk.n_kv, lane);
   const int group = p.pk.group, rows = sp.nq * group;
   const int r0 = sp.tile * kRows;
   if (r0 >= rows) return;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   const int head = blockIdx.x % p.pk.n_kv;
   const int item = (int)(blockIdx.x / p.pk.n_kv);
   const int split = item % p.n_split;
-  const Span sp = span_of(p.pk, true, item / p.n_split, p.k_slots, lane);
+  const Span sp = span_of(p.pk, true, item / p.n_split, p.k_slots, p.pk.n_kv * p.n_split, lane);
   const int j0 = sp.tile * kRows;
   if (j0 >= sp.nk) return;
   const int group = p.pk.group, rows = sp.nq * group;

@@ -115,9 +115,10 @@ __device__ __forceinline__ Span span_of_slot(const Packing& p, bool of_keys, int
 // an eighth further on than the one's before: workgroups go round the XCDs and
 // their shader engines, and where sequences of one length have as many tiles as the
 // round, one engine would get the longest tile of each (the 32 prompts: 73 us).
-// Launches that are resident at once gain too: a CU's second workgroup is then a
-// short one (training on 20, keys not split: 519 and 486 us). Up to one to a CU, the
-// order is all the same.
+// Launches that are resident at once, two workgroups to a CU, take the second half
+// from the shortest on: a CU has a long and a short one (training on 32 of 512, 512
+// workgroups to a kernel: 287 and 275 us). Up to one to a CU, the order is all the
+// same. `each`: workgroups of a tile, heads and splits.
 constexpr int kRankedSeqs = 126;
 constexpr int64_t kRankedTiles = 256;
 
@@ -135,7 +136,8 @@ __device__ __forceinline__ int lanes_upto(int x) {
   return x;
 }
 
-__device__ __forceinline__ Span span_of_rank(const Packing& p, bool of_keys, int rank, int lane) {
+__device__ __forceinline__ Span span_of_rank(const Packing& p, bool of_keys, int rank, int each,
+                                             int lane) {
   const int last = p.n_seq + 1;
   int32_t q0[2], nq[2], k0[2], nk[2], tiles[2], steps[2];
 #pragma unroll
@@ -160,7 +162,9 @@ __device__ __forceinline__ Span span_of_rank(const Packing& p, bool of_keys, int
     return __builtin_amdgcn_readlane(lanes_upto<false>(n), 63);
   };
   Span s{0, 0, 0, 0, kNoTile, 0};
-  if (rank >= total(0)) return s;
+  const int n_tiles = total(0);
+  if (rank >= n_tiles) return s;
+  if (n_tiles * each <= 512 && rank >= 256 / each) rank = n_tiles - 1 - (rank - 256 / each);
   int lo = 0, hi = __builtin_amdgcn_readlane(lanes_upto<true>(max(steps[0], steps[1])), 63) + 1;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -195,8 +199,9 @@ __device__ __forceinline__ Span span_of_rank(const Packing& p, bool of_keys, int
 // The tile of a workgroup; slots are taken from the last one where they count
 // query rows (causal: the last rows of a sequence see the most), from the first
 // where they count keys.
-__device__ __forceinline__ Span span_of(const Packing& p, bool of_keys, int item, int n_slots, int lane) {
-  if (of_keys ? p.ranked_k : p.ranked_q) return span_of_rank(p, of_keys, item, lane);
+__device__ __forceinline__ Span span_of(const Packing& p, bool of_keys, int item, int n_slots, int each,
+                                        int lane) {
+  if (of_keys ? p.ranked_k : p.ranked_q) return span_of_rank(p, of_keys, item, each, lane);
   return span_of_slot(p, of_keys, of_keys ? item : n_slots - 1 - item, lane);
 }
 
