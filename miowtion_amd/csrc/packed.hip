@@ -236,8 +236,9 @@ __device__ __forceinline__ void stage(const lds_u8* kb, const lds_u8* vb, const 
 
 // Bound by power at head_dim 128 (16,384 tokens, 16 heads on 4: 966 us, 1.14
 // PFLOP/s; the matrix cores are busy 68 % of a clock that falls to 1.6 GHz), by the
-// vector units at 64 (four chunks of 512 onto up to 8,192 keys, 32 on 8: 101 us,
-// 0.84 PFLOP/s; about half of their cycles are exponentials). A prompt of 77 is
+// vector units at 64 (four chunks of 512 onto up to 8,192 keys, 32 on 8: 114 us,
+// 0.75 PFLOP/s; about half of their cycles are exponentials, and the longest
+// sequence's tiles end last). A prompt of 77 is
 // launch and latency: 10 us.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
