@@ -190,12 +190,42 @@ def test_many_sequences_of_one_length(n, length):
         pr.check(x, ref, name)
 
 
+def test_graph_of_many_sequences_serves_new_lengths():
+    """Forward and gradients captured once, replayed for lists whose longest
+    sequence lies elsewhere, with rows behind the last one."""
+    n, heads, kv, d, rows = 30, 16, 4, 64, 4096
+    g = torch.Generator().manual_seed(11)
+    q, k, v, dout = (torch.randn(rows, h, d, generator=g).to(BF16).cuda() for h in (heads, kv, kv, heads))
+    cu = pr.offsets([rows // n] * n)
+
+    def step():
+        out, lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+        return [out, lse, *ops_packed.packed_bwd(q, k, v, out, dout, lse, None, cu, cu, True, d ** -0.5)]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in range(4):
+        lens = [int(x) for x in torch.randint(0, 90, (n,), generator=g)]
+        lens[7 * seed] = 1200 + seed
+        cu.copy_(pr.offsets(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = pr.attend(q, k, v, lens, lens, dout=dout)
+        for name, x in zip(('out', 'lse', 'dq', 'dk', 'dv'), got):
+            pr.check(x, ref, name)
+        for x, y in zip(got, step()):  # the same bits as the eager call
+            assert torch.equal(x, y)
+
+
 def test_offsets_out_of_order():
     """Offsets that do not ascend name no sequences: what they give is not said,
     but the calls end, and their inputs stay."""
     g = torch.Generator().manual_seed(3)
-    for n in (2, 5, 61, 62, 63, 200):
-        heads, kv, d = 6, 2, 64
+    for n, heads in ((2, 6), (5, 6), (61, 6), (62, 6), (63, 6), (200, 6), (5, 64), (100, 64), (126, 128)):
+        kv, d = 2, 64
         cu_q, cu_k = (torch.randint(-50, 1000, (n + 1,), generator=g).int().cuda() for _ in range(2))
         q, k, v = (torch.full((rows, h, d), 3.0, dtype=BF16, device='cuda')
                    for rows, h in ((700, heads), (600, kv), (600, kv)))
