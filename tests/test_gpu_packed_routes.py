@@ -190,6 +190,21 @@ def test_many_sequences_of_one_length(n, length):
         pr.check(x, ref, name)
 
 
+@pytest.mark.parametrize('d', [64, 128])
+def test_chunks_of_different_lengths_share_their_keys(d):
+    """A few queries onto many keys: split over the keys, the sequences ordered by
+    their length."""
+    lens_q, lens_k = [64, 1, 70, 50], [1000, 4096, 3001, 3900]
+    heads, kv = 32, 8
+    splits = ops_packed._key_splits(sum(lens_q), sum(lens_k), 4, heads, kv)
+    assert splits > 1 and sum(lens_q) * heads // 128 * splits >= 256
+    q, k, v = _inputs(lens_q, lens_k, heads, kv, d, seed=4, pad_q=2, pad_k=9)
+    out, lse = kernels.packed_attention(q, k, v, pr.offsets(lens_q), pr.offsets(lens_k), return_lse=True)
+    ref = pr.attend(q, k, v, lens_q, lens_k)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+
+
 def test_graph_of_many_sequences_serves_new_lengths():
     """Forward and gradients captured once, replayed for lists whose longest
     sequence lies elsewhere, with rows behind the last one."""
