@@ -579,9 +579,9 @@ int veda_predictor_logits(const float* a, const float* b, int64_t n_heads,
  * or 128; strides (stride_s, stride_h, 1), every row 16-byte aligned.
  * cu_q, cu_k: int32 [n_seq + 1], ascending (offsets outside the rows are
  * clamped to them). lse: fp32 [q_rows, n_heads] contiguous, or NULL.
- * scale: positive and finite. n_split (1 .. 64): workgroups that share the keys
- * of 128 rows; above 1, workspace holds n_split * q_rows * n_heads * (D + 2)
- * floats, 16-byte aligned.
+ * scale: positive and finite. n_heads / n_kv_heads at most 65536. n_split (1 ..
+ * 64): workgroups that share the keys of 128 rows; above 1, workspace holds
+ * n_split * q_rows * n_heads * (D + 2) floats, 16-byte aligned.
  */
 int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                     const void* k, int64_t k_stride_s, int64_t k_stride_h,

@@ -508,6 +508,8 @@ extern "C" int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stri
   VEDA_REQUIRE(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0,
                "packed_fwd: %lld query heads are no multiple of %lld key heads", (long long)n_heads,
                (long long)n_kv_heads);
+  VEDA_REQUIRE(n_heads / n_kv_heads <= kMaxGroup, "packed_fwd: at most %lld query heads to a key head, got %lld",
+               (long long)kMaxGroup, (long long)(n_heads / n_kv_heads));
   VEDA_REQUIRE(q_rows >= 0 && k_rows >= 0 && n_seq >= 0, "packed_fwd: negative size");
   VEDA_REQUIRE(q_rows * n_heads <= 0x7fffff00 && k_rows <= 0x7fffff00 && n_seq < (1 << 20),
                "packed_fwd: q_rows x heads or k_rows past 2^31 - 256, or 2^20 sequences");

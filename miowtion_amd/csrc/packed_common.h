@@ -312,7 +312,11 @@ __device__ __forceinline__ RowLoads<D> load_rows(const uint16_t* x, int64_t stri
   return res;
 }
 
-// 2^32 / group for divisions of less than 2^32 / group by it (0 for one).
+// 2^32 / group, rounded up, for divisions by it (0 for one). The quotient of x is
+// exact for a row of a wave or of a step, at most group + 62, with every group up to
+// 65,536 (each of them tried), and one too large for row group - 1 of 65,537, whose
+// head would wrap below zero.
+constexpr int64_t kMaxGroup = 1 << 16;
 __host__ __device__ inline uint32_t per_group_of(uint32_t group) { return 0xffffffffu / group + 1; }
 
 // Those rows as B operand fragments (lane: row lane % 32, chunk 2 s + lane / 32),

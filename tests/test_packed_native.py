@@ -80,6 +80,28 @@ def test_the_library_refuses_before_any_launch(call, kw, match):
         call(**kw)
 
 
+@pytest.mark.parametrize('group', [(1 << 16) + 1, 70000, 150000])
+def test_more_heads_to_a_key_head_than_the_row_loads_divide_by_are_refused(group):
+    """The forward and the backward find a row's token by a product with 2^32 / group,
+    which is exact up to 65,536 and wrong for row group - 1 of the first past it."""
+    with pytest.raises(ValueError, match='query heads to a key head'):
+        _fwd(heads=group, kv=1, rows=1)
+    with pytest.raises(ValueError, match='query heads to a key head'):
+        _bwd(heads=group, kv=1, rows=1)
+
+
+def test_the_row_loads_division_is_exact_for_every_group_that_is_taken():
+    """A product with ceil(2^32 / group) can only be too large, and first at the rows
+    before a multiple of the group; rows go up to group + 63."""
+    for group in range(2, (1 << 16) + 1):
+        m = 0xffffffff // group + 1
+        # the excess grows with the row, so the last such row decides
+        x = (group + 63) // group * group - 1
+        assert x * m >> 32 == x // group, group
+    group = (1 << 16) + 1
+    assert (group - 1) * (0xffffffff // group + 1) >> 32 == 1
+
+
 def test_calls_without_work_launch_nothing():
     _fwd(rows=0)
     _append(rows=0)
