@@ -599,7 +599,9 @@ int veda_packed_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
  * P^T dout, dk and dv summed over the query heads of a key head. Rows of no
  * sequence and rows that see (or are seen by) nothing get zeros. Every row is
  * written by one workgroup: the same bits on every call.
- * out, lse: what the forward gave (lse [q_rows, n_heads] contiguous). dlse: fp32
+ * Strides of rows of q, k, v and dout, and with several query heads to a key head
+ * those of heads of q and dout, below 2^24 (with more than 64, below 2^30 over all
+ * of them). out, lse: what the forward gave (lse [q_rows, n_heads] contiguous). dlse: fp32
  * as lse, or NULL. dq [q_rows, n_heads, D], dk, dv [k_rows, n_kv_heads, D]:
  * bf16 contiguous. n_split (1 .. 64): workgroups that share the query rows of a key
  * tile. workspace: 16-byte aligned, 1,024 bytes for each of n_kv_heads * (q_rows *

@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
 
   // The steps' rows are loaded in turn: t0, rem are the next step's first token
   // and head. Row x from there is token x / group by a product with 2^32 / group
-  // (exact: x < 64 + group, and x group < 2^32).
+  // (exact: x < 63 + group, kMaxGroup).
   int t0 = 0, rem = 0;
   if (n_steps > 0) {
     t0 = (int)((int64_t)64 * top / group);
@@ -594,7 +594,10 @@ extern "C" int veda_packed_bwd(
                    rows16(dv, 0, 0),
                "packed_bwd: q, k, v, out, dout and gradient rows must be 16-byte aligned");
   // the LDS loads address a 64-row step with 32-bit byte offsets
-  const int64_t strides[] = {q_stride_s, q_stride_h, k_stride_s, v_stride_s, do_stride_s, do_stride_h};
+  // (of one key head's rows: with one query head to each, no head stride)
+  const bool heads = n_heads > n_kv_heads;
+  const int64_t strides[] = {q_stride_s, k_stride_s, v_stride_s, do_stride_s, heads ? q_stride_h : 0,
+                             heads ? do_stride_h : 0};
   for (int64_t s : strides)
     VEDA_REQUIRE(s >= 0 && s < (1 << 24), "packed_bwd: stride negative or too large");
   BwdArgs p{};
@@ -602,7 +605,8 @@ extern "C" int veda_packed_bwd(
                  (int32_t)(n_heads / n_kv_heads), causal ? 1 : 0,
                  ranked(n_seq, q_rows * n_heads / kRows),
                  ranked(n_seq, k_rows * n_kv_heads / kRows * n_split)};
-  VEDA_REQUIRE(p.pk.group <= 65000, "packed_bwd: at most 65000 query heads to a key head");
+  VEDA_REQUIRE(p.pk.group <= kMaxGroup, "packed_bwd: at most %lld query heads to a key head, got %lld",
+               (long long)kMaxGroup, (long long)p.pk.group);
   VEDA_REQUIRE(p.pk.group <= 64 || (q_stride_h * p.pk.group < (1 << 30) &&
                                     do_stride_h * p.pk.group < (1 << 30)),
                "packed_bwd: the heads of a group are too far apart");

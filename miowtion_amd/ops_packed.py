@@ -133,6 +133,17 @@ def _splits(k_rows: int, kv_heads: int, walk: int = 1 << 14) -> int:
     return max(min(-(-want // tiles), walk // 256, 16), 1)
 
 
+def _near(t: torch.Tensor, at: list, group: int, device: int):
+    """`at` ([pointer, row stride, head stride] of t) if the dk and dv kernel can load
+    rows in these strides, which it addresses by 32-bit offsets within a step of 64;
+    else a contiguous copy and its own, which it can below 2^24 values a row."""
+    _, s, h = at
+    if s < 1 << 24 and (group == 1 or h < 1 << 24) and (group <= 64 or h * group < 1 << 30):
+        return t, at
+    t = t.contiguous()
+    return t, list(_rows('q', t, device)[1:])
+
+
 @_custom_op('veda::packed_bwd', mutates_args=())
 def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                dout: torch.Tensor, lse: torch.Tensor, dlse: torch.Tensor | None,
@@ -141,11 +152,14 @@ def packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Ten
     """[dq, dk, dv] of packed_fwd, from its out and lse."""
     dev, shape, tensors, sizes = _check_packed(q, k, v, cu_q, cu_k, scale)
     rows, heads, d = shape
+    group = heads // k.shape[1]
+    q, tensors[:3] = _near(q, tensors[:3], group, dev)
     for name, t in (('out', out), ('dout', dout)):
         got, *more = _rows(name, t, dev)
         if got != shape:
             raise ValueError(f'{name} {list(got)} must be as q {list(shape)}')
         tensors += more
+    dout, tensors[-3:] = _near(dout, tensors[-3:], group, dev)
     for name, t in (('lse', lse), ('dlse', dlse)):
         if t is not None and (t.dtype is not _F32 or t.shape != (rows, heads)
                               or not t.is_contiguous() or t.get_device() != dev):

@@ -60,6 +60,8 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
+        if q.shape[0] > 1 and math.prod(q.shape[1:]) >= 1 << 24:  # refused here, not by the backward
+            raise ValueError(f'gradients need fewer than 2^24 values in a row of q, got {list(q.shape)}')
         out, lse = ops_packed.packed_fwd(q, k, v, cu_q, cu_k, causal, scale, True)
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
         ctx.causal, ctx.scale = causal, scale
@@ -86,8 +88,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
 
     Args:
         q: [Tq, H, D] bf16, D 64 or 128; rows in any strides on 16-byte boundaries.
-        k, v: [Tk, Hkv, D] bf16, H a multiple of Hkv: query head h attends with
-            key head h // (H // Hkv).
+            For gradients H * D is below 2^24, and a q whose strides reach 2^24
+            (beyond 64 heads to a key head, 2^30 over those) is copied.
+        k, v: [Tk, Hkv, D] bf16, H a multiple of Hkv, at most 65,536 times: query
+            head h attends with key head h // (H // Hkv). Row strides below 2^24.
         cu_q: int32 [B + 1], ascending: sequence b has the rows cu_q[b] ..
             cu_q[b + 1] - 1 of q. Offsets are not checked (they stay on the GPU);
             ones outside the rows are clamped to them.

@@ -178,6 +178,66 @@ def test_graph_of_forward_and_backward():
             pr.check(x, ref, name)
 
 
+FAR = [
+    # heads, kv, d, row stride, head stride: past what a step's 32-bit offsets reach
+    (4, 2, 64, None, 1 << 24),
+    (2, 2, 128, None, (1 << 24) + 128),          # a head to a group: no head offset in a step
+    (2, 1, 128, 1 << 24, None),
+    (65, 1, 64, None, (1 << 24) - 64),           # in reach each, not over the group
+]
+
+
+@pytest.mark.parametrize('case', FAR, ids=lambda c: f'{c[0]}-{c[1]}-{c[2]}')
+def test_queries_in_strides_past_32_bit_offsets(case):
+    """Every layout of q that the forward takes has gradients, the same bits as a
+    contiguous q's."""
+    heads, kv, d, s, h = case
+    lens = [7, 4] if s else [70, 33]
+    q, k, v = _inputs(lens, lens, heads, kv, d, seed=9)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    s, h = s or d, h or d
+    room = torch.empty((sum(lens) - 1) * s + (heads - 1) * h + d, dtype=q.dtype, device='cuda')
+    far = room.as_strided(q.shape, (s, h, 1))
+    far.copy_(q)
+    print(f'q in strides {far.stride()}', flush=True)
+    cu = pr.offsets(lens)
+    want = _grads(q, k, v, cu, None, True, dout)
+    for a, b in zip(_grads(far, k, v, cu, None, True, dout), want):
+        assert torch.equal(a, b)
+    ref = pr.attend(q, k, v, lens, lens, dout=dout)
+    for name, x in zip(('dq', 'dk', 'dv'), want):
+        pr.check(x, ref, name)
+    # an output gradient laid out so, straight into the op
+    out, lse = kernels.packed_attention(q, k, v, cu, return_lse=True)
+    far.copy_(dout)
+    for a, b in zip(ops_packed.packed_bwd(q, k, v, out, far, lse, None, cu, cu, True, d ** -0.5), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('group', [65535, 65536])
+def test_the_largest_groups(group):
+    """Without a mask the heads of one key head are rows of one head."""
+    print(f'{group} query heads to a key head', flush=True)
+    lens, d = [2, 1], 64
+    q, k, v = _inputs(lens, lens, group, 1, d, seed=10)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    cu = pr.offsets(lens)
+    out = kernels.packed_attention(q, k, v, cu, causal=False)
+    ref = pr.attend(q.view(-1, 1, d), k, v, [n * group for n in lens], lens, False, dout=dout.view(-1, 1, d))
+    pr.check(out.view(-1, 1, d), ref, 'out')
+    for name, x in zip(('dq', 'dk', 'dv'), _grads(q, k, v, cu, None, False, dout)):
+        pr.check(x.view(-1, 1, d), ref, name)
+
+
+def test_rows_too_wide_for_gradients_are_refused_by_the_forward():
+    q = torch.zeros(2, 1 << 17, 128, dtype=torch.bfloat16, device='cuda')
+    k = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device='cuda')
+    cu = pr.offsets([2])
+    assert (kernels.packed_attention(q, k, k, cu) == 0).all()
+    with pytest.raises(ValueError, match='gradients need'):
+        kernels.packed_attention(q.requires_grad_(), k, k, cu)
+
+
 def test_only_some_inputs_require_grad_and_second_order_is_refused():
     lens = [40]
     q, k, v = _inputs(lens, lens, 2, 2, 64)

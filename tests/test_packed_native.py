@@ -90,6 +90,15 @@ def test_more_heads_to_a_key_head_than_the_row_loads_divide_by_are_refused(group
         _bwd(heads=group, kv=1, rows=1)
 
 
+def test_rows_that_a_step_cannot_address_are_copied():
+    at = 1 << 24
+    for group, stride, copied in ((1, (64, at, 1), False), (2, (64, at, 1), True), (1, (at, 64, 1), True),
+                                  (2, (64, at - 64, 1), False), (65, (64, at - 64, 1), True)):
+        t = torch.empty(1, dtype=torch.bfloat16).expand(2, 65, 64).as_strided((1, 1, 1), (1, 1, 1)).expand(2, 65, 64)
+        got, (_, s, h) = ops_packed._near(t, [0, *stride[:2]], group, -1)
+        assert ((s, h) == (65 * 64, 64)) == copied and got.is_contiguous() == copied
+
+
 def test_the_row_loads_division_is_exact_for_every_group_that_is_taken():
     """A product with ceil(2^32 / group) can only be too large, and first at the rows
     before a multiple of the group; rows go up to group + 63."""
