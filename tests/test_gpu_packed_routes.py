@@ -92,6 +92,20 @@ def test_rows_that_share_memory_are_not_written():
     assert torch.equal(got[:, 0], got[:, 1])
 
 
+def test_exponents_that_share_memory_are_not_written():
+    cache, table, lengths, k, v, start, cu = _cache(torch.float8_e4m3fn)
+    flat = [t[:, :, :1].expand(-1, -1, 2) for t in cache[2:]]
+    for bad in (cache._replace(k_exp=flat[0], v_exp=flat[1]), cache._replace(v_exp=cache.k_exp),
+                cache._replace(v=cache.k)):
+        with pytest.raises(ValueError, match='share memory'):
+            kernels.cache_append_(bad, k, v, cu, table, start)
+    # reading them is fine
+    kernels.cache_append_(cache, k, v, cu, table, start)
+    got, _ = kernels.cache_gather(cache._replace(k_exp=flat[0], v_exp=flat[1]), cu, table, 57)
+    want, _ = kernels.cache_gather(cache, cu, table, 57)
+    assert torch.equal(got[:, 0], want[:, 0])
+
+
 def test_calls_on_two_streams_at_once():
     lens = [700, 300]
     cases = [_inputs(lens, lens, 8, 2, 128, seed=s) for s in range(4)]

@@ -197,3 +197,26 @@ def test_reference_of_held_rows_agrees_with_torch():
     assert torch.equal((x.double() / unit).float().to(torch.float8_e4m3fn).double() * unit, values)
     top = x.double().abs().amax(-1, keepdim=True) / unit
     assert (top <= 448).all() and (top > 224).all()
+
+
+def _shared_caches():
+    """(cache, what of it shares memory): caches whose rows cannot all be written."""
+    cache = kernels.paged_cache(2, 16, 2, 64, torch.float8_e4m3fn, device='cpu')
+    heads, rows = cache.k_exp[:, :, :1].expand(-1, -1, 2), cache.k_exp[:, :1].expand(-1, 16, -1)
+    for exp in (heads, rows):
+        yield cache._replace(k_exp=exp, v_exp=exp.clone().as_strided(exp.shape, exp.stride()))
+        yield cache._replace(v_exp=exp, k_exp=exp.clone().as_strided(exp.shape, exp.stride()))
+    yield cache._replace(v_exp=cache.k_exp)
+    yield cache._replace(v=cache.k)
+    plain = kernels.paged_cache(2, 16, 2, 64, device='cpu')
+    yield plain._replace(v=plain.k)
+    yield kernels.PagedCache(*(t[:1].expand(2, -1, -1, -1) for t in plain[:2]))
+
+
+def test_caches_that_share_memory_are_not_written():
+    k, cu = _cpu(4, 2, 64), _cpu(2, dtype=torch.int32)
+    table, one = _cpu(1, 2, dtype=torch.int32), _cpu(1, dtype=torch.int32)
+    append = ops_packed.cache_append_._fn  # what runs behind the refusal of CPU tensors
+    for cache in _shared_caches():
+        with pytest.raises(ValueError, match='share memory'):
+            append(*cache, k, k, cu, table, one)
