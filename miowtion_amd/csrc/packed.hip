@@ -38,11 +38,15 @@ struct FwdArgs {
   uint32_t per_group;
 };
 
-// A row whose O came out with an infinity or a NaN, again, key by key: a key
-// that the row does not see, or whose probability is zero, adds nothing
-// whatever its V holds (a product with a zero probability makes a NaN of it).
-// All lanes of the wave work on the row; lane l has head-dims l and l + 64. To
-// out as bf16, or, where part is given, there in 32 bits.
+// A row whose O came out with a NaN though its sum of weights has none, again, key
+// by key: a key that the row does not see, or whose probability is zero, adds
+// nothing whatever its V holds (a product with a zero probability makes a NaN of an
+// infinity or a NaN). All lanes of the wave work on the row; lane l has head-dims l
+// and l + 64. To out as bf16, or, where part is given, there in 32 bits.
+// A row costs some 200 times its share of the walk (4,096 tokens, 8 heads on 2: all
+// rows 14 ms, the walk 67 us), so rows that the walk has right are left out: an
+// infinity is one of a key with a weight, and a sum of weights that is NaN, as any
+// score that is NaN makes it, gives a NaN in every column either way.
 template <int D>
 __device__ __noinline__ void redo_row(const uint16_t* q, const uint16_t* k, const uint16_t* v,
                                       int64_t ks, int64_t vs, int limit, float c, float mu, float inv,
@@ -399,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
 #pragma unroll
   for (int t = 0; t < T::kT; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[t][e]) < INFINITY);
-  const uint64_t bad_lanes = __ballot(bad);
+    for (int e = 0; e < 16; ++e) bad |= o[t][e] != o[t][e];
+  const uint64_t bad_lanes = __ballot(bad && l == l);
   uint32_t bad_rows = (uint32_t)bad_lanes | (uint32_t)(bad_lanes >> 32);
   auto redo = [&](uint32_t which) {
     while (which != 0) {

@@ -159,6 +159,73 @@ def test_values_behind_the_mask_do_not_reach_a_row(d):
     assert torch.equal(out[290:], clean[290:]) and torch.equal(out[:90], clean[:90])
 
 
+def _time(fn, *args):
+    """The least of five times, in us."""
+    fn(*args)
+    times = []
+    for _ in range(5):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        fn(*args)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(begin.elapsed_time(end) * 1e3)
+    return min(times)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_what_every_row_sees_takes_no_longer(d):
+    """A key or a value that is not finite where every row sees it: not a case for
+    the way that forms a row key by key, which takes 200 times as long."""
+    lens = [4096, 300]
+    q, k, v = _inputs(lens, lens, 8, 2, d, seed=8)
+    cu = pr.offsets(lens)
+
+    def attend(k, v):
+        return kernels.packed_attention(q, k, v, cu, return_lse=True)
+
+    clean, clean_lse = attend(k, v)
+    plain = _time(attend, k, v)
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[0, 0] = math.nan
+    bad_v[0, 1, 3] = -math.inf
+    out, lse = attend(bad_k, v)
+    assert torch.isnan(out[:4096, :4]).all() and torch.isnan(lse[:4096, :4]).all()
+    assert torch.equal(out[4096:], clean[4096:]) and torch.equal(lse[4096:], clean_lse[4096:])
+    assert torch.equal(out[:, 4:], clean[:, 4:]) and torch.equal(lse[:, 4:], clean_lse[:, 4:])
+    took = _time(attend, bad_k, v)
+    print(f'{plain:.0f} us, with a key that is NaN {took:.0f}', flush=True)
+    assert took < 10 * plain
+    out, lse = attend(k, bad_v)
+    assert (out[:4096, 4:, 3] == -math.inf).all() and torch.equal(lse, clean_lse)
+    out[:4096, 4:, 3] = clean[:4096, 4:, 3]
+    assert torch.equal(out, clean)
+    took = _time(attend, k, bad_v)
+    print(f'{plain:.0f} us, with a value that is infinite {took:.0f}', flush=True)
+    assert took < 10 * plain
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_a_score_that_is_not_a_number_in_some_splits(d):
+    """Keys shared by workgroups: the NaN of one split's sum of weights reaches every
+    column, and where another's V is behind the mask as well."""
+    lens_q, lens_k = [130, 3], [6000, 4000]
+    assert ops_packed._key_splits(133, 10000, 2, 4, 2) > 1
+    q, k, v = _inputs(lens_q, lens_k, 4, 2, d, seed=12)
+    cu_q, cu_k = pr.offsets(lens_q), pr.offsets(lens_k)
+    ref = pr.attend(q, k, v, lens_q, lens_k)
+    k[40, 0, 1] = math.nan
+    v[5950, 0, 2] = math.inf   # seen by the rows from 80 on
+    v[5950, 1, 2] = math.inf
+    out, lse = kernels.packed_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    assert torch.isnan(out[:130, :2]).all() and torch.isnan(lse[:130, :2]).all()
+    assert (out[80:130, 2:, 2] == math.inf).all()
+    out[:130, :2], lse[:130, :2] = ref['out'][:130, :2].to(out.dtype), ref['lse'][:130, :2].float()
+    out[80:130, 2:, 2] = ref['out'][80:130, 2:, 2].to(out.dtype)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+
+
 def test_strides_and_shared_storage():
     lens = [130, 61]
     g = torch.Generator().manual_seed(1)
