@@ -24,6 +24,15 @@ import torch
 
 H = 2.0 ** -8
 R = 2.0 ** -11
+# A gradient's distance from 64 bits by its norm, a head's: those bounds are worst
+# cases of every value, and leave room for a D that is off. A bf16 rounding is even
+# over a step of 2^-7 2^e, 2^-7 / sqrt(12) by its square mean, of values m 2^e whose
+# square mean is 1.47 2^e where log m is even: 1.5e-3. Two are in a gradient, dS's
+# and its own, of which dS's meets terms that may cancel: 2.1e-3 to 2.7e-3 by
+# `gradients_as_rounded` at thousands of keys, and 1.5 times the two together here.
+# With D from the bf16 out as it is, or without what the rounded dS sum to taken off,
+# keys with a direction in common give 4e-3 to 2e-2.
+NORM = 3.5e-3
 
 
 def offsets(lens, device='cuda'):
@@ -87,6 +96,56 @@ def attend(q, k, v, lens_q, lens_k, causal=True, scale=None, dout=None, dlse=Non
         for name in ('dq', 'dk', 'dv'):
             res[name + '_tol'] += H * res[name].abs() + 1e-30
     return res
+
+
+def leaning(n, heads, kv, d, seed, device='cuda'):
+    """q, k, v, dout in bf16 and dlse of n tokens, queries and keys with a direction in
+    common, as they have it after normalisation."""
+    g = torch.Generator().manual_seed(seed)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g)
+
+    shared = rand(1, 1, d)
+    ts = (rand(n, heads, d) + 0.7 * shared, rand(n, kv, d) + 0.7 * rand(n, kv, 1) * shared,
+          rand(n, kv, d), rand(n, heads, d))
+    return [t.to(torch.bfloat16).to(device) for t in ts] + [rand(n, heads).to(device)]
+
+
+def gradients_as_rounded(q, k, v, dout, dlse=None, take_off=True, mend=True, sign=1):
+    """(dq, dk) of one causal sequence in 64 bits but for the roundings to bf16 of P, dS,
+    out and the results. take_off: what the rounded dS of a row sum to beside dlse is
+    taken off its dq, times P K; mend: D of dk is mended by what the exact ones sum to;
+    sign: of dlse in that sum."""
+    def bf16(x):
+        return x.to(torch.bfloat16).double()
+
+    q, k, v, dout = (t.double() for t in (q, k, v, dout))
+    n, heads, d = q.shape
+    dq, dk = torch.zeros_like(q), torch.zeros_like(k)
+    see = torch.ones(n, n, dtype=torch.bool, device=q.device).tril()
+    for h in range(heads):
+        kh, vh = (t[:, h // (heads // k.shape[1])] for t in (k, v))
+        a = (q[:, h] @ kh.t() * d ** -0.5).masked_fill(~see, -math.inf)
+        p = torch.softmax(a, -1)
+        dl = 0.0 * p[:, 0] if dlse is None else dlse[:, h].double()
+        dd = (dout[:, h] * bf16(bf16(p) @ vh)).sum(-1) - dl
+        dp = dout[:, h] @ vh.t()
+        ds = p * (dp - dd[:, None])
+        x = bf16(ds) @ kh
+        if take_off:
+            x += (sign * dl - bf16(ds).sum(-1))[:, None] * (bf16(p) @ kh)
+        dq[:, h] = bf16(d ** -0.5 * x)
+        if mend:
+            ds = p * (dp - (dd + ds.sum(-1) - dl)[:, None])
+        dk[:, h // (heads // k.shape[1])] += d ** -0.5 * (bf16(ds).t() @ q[:, h])
+    return dq, bf16(dk)
+
+
+def distance(got, want):
+    """The largest of the heads' distances by norm, relative."""
+    off = (got.double() - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2))
+    return off.max().item()
 
 
 def check(got, ref, name):

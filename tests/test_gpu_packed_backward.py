@@ -79,6 +79,23 @@ def test_gradients_are_the_differences():
         assert (mine - diff).abs() <= tol, (name, mine.item(), diff.item(), tol.item())
 
 
+@pytest.mark.parametrize('through_lse', [False, True])
+@pytest.mark.parametrize('d', [64, 128])
+def test_distance_of_long_sequences_by_norm(d, through_lse):
+    """Thousands of keys with a direction in common: what the rounded dS of a row sum
+    to would meet their mean."""
+    n, heads, kv = 3001, 4, 2
+    q, k, v, dout, dlse = pr.leaning(n + 70, heads, kv, d, seed=0)
+    dlse = dlse if through_lse else None
+    got = _grads(q, k, v, pr.offsets([n, 70]), None, True, dout, dlse)
+    ref = pr.attend(q, k, v, [n, 70], [n, 70], dout=dout, dlse=dlse)
+    for name, x in zip(('dq', 'dk', 'dv'), got):
+        off = pr.distance(x[:n], ref[name][:n])
+        print(f'{name} {off:.2e}', flush=True)
+        assert off < pr.NORM
+        pr.check(x, ref, name)
+
+
 def test_rows_and_keys_of_no_sequence_get_zeros():
     lens = [50, 200]
     q, k, v = _inputs(lens, lens, 4, 2, 128, pad_q=150, pad_k=140)

@@ -190,6 +190,26 @@ def test_reference_agrees_with_torch():
         torch.testing.assert_close(ref[name], x)
 
 
+@pytest.mark.parametrize('through_lse', [False, True])
+@pytest.mark.parametrize('d', [64, 128])
+def test_the_bound_by_norm_tells_the_row_sums_correction(d, through_lse):
+    """Gradients rounded as the kernels round them are within it, and past it without
+    each part of the correction, for the long sequence that the GPU's test has."""
+    n = 3001
+    q, k, v, dout, dlse = (t[:n] for t in pr.leaning(n + 70, 4, 2, d, seed=0, device='cpu'))
+    dlse = dlse if through_lse else None
+    ref = pr.attend(q, k, v, [n], [n], dout=dout, dlse=dlse)
+    dq, dk = pr.gradients_as_rounded(q, k, v, dout, dlse)
+    assert pr.distance(dq, ref['dq']) < pr.NORM and pr.distance(dk, ref['dk']) < pr.NORM
+    dq, _ = pr.gradients_as_rounded(q, k, v, dout, dlse, take_off=False)
+    assert pr.distance(dq, ref['dq']) > pr.NORM
+    _, dk = pr.gradients_as_rounded(q, k, v, dout, dlse, mend=False)
+    assert pr.distance(dk, ref['dk']) > pr.NORM
+    if through_lse:
+        dq, _ = pr.gradients_as_rounded(q, k, v, dout, dlse, sign=-1)
+        assert pr.distance(dq, ref['dq']) > pr.NORM
+
+
 def test_reference_of_held_rows_agrees_with_torch():
     x = torch.randn(200, 64, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16) * 30
     values, byte = pr.held(x)
