@@ -30,6 +30,7 @@ R = 2.0 ** -11
 # square mean is 1.47 2^e where log m is even: 1.5e-3. Two are in a gradient, dS's
 # and its own, of which dS's meets terms that may cancel: 2.1e-3 to 2.7e-3 by
 # `gradients_as_rounded` at thousands of keys, and 1.5 times the two together here.
+# An out has P's, whose terms do not cancel more, and its own.
 # With D from the bf16 out as it is, or without what the rounded dS sum to taken off,
 # keys with a direction in common give 4e-3 to 2e-2.
 NORM = 3.5e-3

@@ -98,6 +98,24 @@ def test_keys_shared_by_workgroups(case):
     pr.check(rest, ref, 'out')
 
 
+@pytest.mark.parametrize('case', SPLIT + [([3000, 1000], None, 4, 2, 64, True), ([3000, 1000], None, 4, 2, 128, False)],
+                         ids=lambda c: f'{len(c[0])}x{max(c[0])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}')
+def test_distance_by_norm(case):
+    """Thousands of keys of like weight leave an out of some hundredths: the bound of a
+    value, of the size of v, would let a split's sums go."""
+    lens_q, lens_k, heads, kv, d, causal = case
+    lens_k = lens_k or lens_q
+    print(f'packed forward by norm {case}', flush=True)
+    q, k, v = _inputs(lens_q, lens_k, heads, kv, d, seed=2)
+    out = kernels.packed_attention(q, k, v, pr.offsets(lens_q), pr.offsets(lens_k), causal=causal)
+    ref = pr.attend(q, k, v, lens_q, lens_k, causal)['out']
+    first = 0
+    for n in lens_q:
+        rows, first = slice(first, first + n), first + n
+        off = (out[rows].double() - ref[rows]).norm(dim=(0, 2))
+        assert (off <= pr.NORM * ref[rows].norm(dim=(0, 2))).all(), off
+
+
 def test_scale_and_large_scores():
     lens = [200, 33]
     q, k, v = _inputs(lens, lens, 4, 2, 128, seed=3)

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from miowtion_amd import kernels
+from miowtion_amd import _native, kernels, ops_packed
 from tests import packed_reference as pr
 
 pytestmark = pytest.mark.gpu
@@ -208,6 +208,77 @@ def test_one_token(case, dtype):
     pr.check(out, ref, 'out')
     pr.check(lse, ref, 'lse')
     assert torch.equal(out, kernels.paged_attention(q, cache, table, lengths))
+
+
+def _near_by_norm(out, ref):
+    """Each sequence's out by norm: thousands of keys of like weight leave an out of
+    some hundredths, and the bound of a value, of the size of v, lets a part go."""
+    off = (out.double() - ref['out']).norm(dim=(1, 2))
+    assert (off <= pr.NORM * ref['out'].norm(dim=(1, 2))).all(), off
+
+
+PARTS = [
+    # lens, heads, kv, d, page, width: more than 64 parts, joined by eight waves: some
+    # of them without a part, parts that do not divide by eight, more than 512
+    ([1, 16500, 0, 9000], 5, 1, 128, 16, 1100),
+    ([1, 16500, 0, 9000], 5, 1, 64, 16, 1300),
+    ([17000, 30], 17, 1, 64, 64, 300),
+    ([33000, 16640], 3, 3, 128, 256, None),
+    ([600001, 70000], 3, 1, 64, 32, None),
+]
+
+
+@pytest.mark.parametrize('dtype', [BF16, E4M3], ids=['bf16', 'e4m3'])
+@pytest.mark.parametrize('case', PARTS, ids=lambda c: f'{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-{c[3]}-{c[4]}')
+def test_one_token_of_many_parts(case, dtype):
+    lens, heads, kv, d, page, width = case
+    cache, table, k, v = _filled(lens, page, kv, d, dtype, width=width)
+    capacity = table.shape[1] * page
+    parts = -(-capacity // ops_packed._chunk(len(lens), kv, heads // kv, capacity, page))
+    print(f'one token of many parts {case} {dtype}: {parts}', flush=True)
+    assert parts > (512 if max(lens) > 500000 else 64)
+    q = torch.randn(len(lens), heads, d, generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    lengths = torch.tensor(lens, dtype=torch.int32, device='cuda')
+    out, lse = kernels.paged_attention(q, cache, table, lengths, return_lse=True)
+    ref = pr.attend(q, k, v, [1] * len(lens), lens)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+    _near_by_norm(out, ref)
+    assert torch.equal(out, kernels.paged_attention(q, cache, table, lengths))
+    # a page of the longest sequence outside the cache
+    b = lens.index(max(lens))
+    first = sum(lens[:b])
+    at = 300 // page
+    table[b, at] = -1
+    seen = torch.ones(lens[b], dtype=torch.bool)
+    seen[at * page:(at + 1) * page] = False
+    rows = slice(first, first + lens[b])
+    ref = pr.attend(q[b:b + 1], k[rows][seen], v[rows][seen], [1], [int(seen.sum())])
+    out, lse = kernels.paged_attention(q, cache, table, lengths, return_lse=True)
+    pr.check(out[b:b + 1], ref, 'out')
+    pr.check(lse[b:b + 1], ref, 'lse')
+
+
+@pytest.mark.parametrize('dtype', [BF16, E4M3], ids=['bf16', 'e4m3'])
+@pytest.mark.parametrize('pages', [66, 128])
+def test_chunks_of_more_pages_than_a_wave_has_lanes(pages, dtype):
+    """Through the library's entry point: the ops ask for 64 pages to a chunk at most."""
+    lens, heads, kv, d, page, width = [3000, 1, 0, 4999], 4, 2, 128, 16, 320
+    cache, table, k, v = _filled(lens, page, kv, d, dtype, width=width)
+    q = torch.randn(len(lens), heads, d, generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    lengths = torch.tensor(lens, dtype=torch.int32, device='cuda')
+    out, lse = torch.empty_like(q), torch.empty(len(lens), heads, device='cuda')
+    chunk = pages * page
+    work = torch.empty(len(lens) * heads * -(-width * page // chunk) * (d + 4), device='cuda')
+    args, sizes = ops_packed._check_cache(*cache, table, kv, d, 0)
+    print(f'chunks of {pages} pages {dtype}', flush=True)
+    _native.call('veda_paged_fwd', q.data_ptr(), heads * d, d, len(lens), heads, kv, d, *args, *sizes,
+                 lengths.data_ptr(), d ** -0.5, chunk, out.data_ptr(), heads * d, d, lse.data_ptr(),
+                 work.data_ptr(), 4 * work.numel(), torch.cuda.current_stream().cuda_stream)
+    ref = pr.attend(q, k, v, [1] * len(lens), lens)
+    pr.check(out, ref, 'out')
+    pr.check(lse, ref, 'lse')
+    _near_by_norm(out, ref)
 
 
 def test_lengths_and_pages_out_of_range():
