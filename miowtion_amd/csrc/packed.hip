@@ -82,6 +82,9 @@ __device__ __noinline__ void redo_row(const uint16_t* q, const uint16_t* k, cons
 }
 
 // ---------------------------------------------------------------------------
+// The walk of the dense forward (attention.hip, head_dim 128 alone: what is mended in
+// one is for the other too), with its own tiles and masks.
+//
 // A stage works on three consecutive 32-key sub-blocks at once: the score
 // products of sub-block n + 1 (QK: K rows at `kb` into sn), the softmax of n (SM:
 // scores sp into the packed probabilities pn) and the P V products of n - 1 (PV: V
@@ -239,9 +242,9 @@ __device__ __forceinline__ void stage(const lds_u8* kb, const lds_u8* vb, const 
 }
 
 // Bound by power at head_dim 128 (16,384 tokens, 16 heads on 4: 966 us, 1.14
-// PFLOP/s; the matrix cores are busy 68 % of a clock that falls to 1.6 GHz), by the
-// vector units at 64 (four chunks of 512 onto up to 8,192 keys, 32 on 8: 114 us,
-// 0.75 PFLOP/s; about half of their cycles are exponentials, and the longest
+// PFLOP/s; the matrix cores are busy 69 % of a clock that falls to 1.6 GHz), by the
+// vector units at 64 (four chunks of 512 onto up to 8,192 keys, 32 on 8: 106 us a
+// call, 0.80 PFLOP/s; about half of their cycles are exponentials, and the longest
 // sequence's tiles end last). A prompt of 77 is
 // launch and latency: 10 us.
 template <int D>
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
 }
 
 // The splits of a row joined: D / 4 threads a row, four head-dims each. Bound by
-// memory (2,048 rows of 32 heads, two splits, head_dim 64: 9.0 us, 4.8 TB/s).
+// memory (512 rows of 32 heads, four splits, head_dim 128: 7.8 us, 4.9 TB/s).
 template <int D>
 __global__ void __launch_bounds__(256) packed_merge_kernel(FwdArgs p) {
   const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;

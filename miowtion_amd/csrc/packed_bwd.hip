@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[Tile<D>::kT], flo
 }
 
 // Four products a pair. Bound by power as the forward is: 8,192 tokens, 28 heads on
-// 4, 829 us, 1.16 PFLOP/s, the matrix cores busy 62 % of 1.8 GHz.
+// 4, 847 us, 1.14 PFLOP/s, the matrix cores busy 62 % of 1.8 GHz.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   using T = Tile<D>;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_dq_kernel(BwdArgs p) {
   });
 }
 
-// Four products a pair: the same tokens 876 us, 1.10 PFLOP/s, busy 58 %.
+// Four products a pair: the same tokens 889 us, 1.08 PFLOP/s, busy 58 %.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) packed_dkv_kernel(BwdArgs p) {
   using T = Tile<D>;

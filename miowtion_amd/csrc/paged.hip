@@ -140,7 +140,7 @@ __device__ __forceinline__ u32x2 encode8(u32x4 x, uint32_t& byte) {
 }
 
 // Bound by memory where there are rows enough (4,096 rows of 8 key heads in bf16:
-// 9.0 us, 3.7 TB/s), by its start at a row for each of 32 sequences (7.6 us).
+// 9.0 us, 3.7 TB/s), by its start at a row for each of 32 sequences (7.4 us).
 template <int D, bool F8>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs p) {
   constexpr int kLanes = D / 8, kRowsAtOnce = 64 / kLanes;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs p) {
 
 // ---------------------------------------------------------------------------
 // Reading back. A wave takes one row of the packed result, as above. Bound by
-// memory (52,769 rows of 8 key heads in bf16: 432 MB in 76.8 us, 5.6 TB/s).
+// memory (52,769 rows of 8 key heads in bf16: 432 MB in 77.8 us, 5.6 TB/s).
 
 struct GatherArgs {
   Pages kp, vp;
@@ -271,7 +271,7 @@ __device__ __forceinline__ int length_of(const TokenArgs& p, int b) {
   return min(max(p.lengths[b], 0), p.tab.width << p.tab.shift);
 }
 
-// Bound by memory: four tokens over 386,613 positions in bf16, 8 key heads, 277 us,
+// Bound by memory: four tokens over 386,613 positions in bf16, 8 key heads, 279 us,
 // 5.7 TB/s; 64 over 73,366 in e4m3 33.8 us, 4.5 TB/s, the start and the uneven end
 // of a short kernel among it; one over 1,500, 5.4 us of latency.
 template <int D, bool F8, int W>
