@@ -231,12 +231,13 @@ def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exp: torch.Ten
         raise ValueError(f'k {[rows, heads, d]} and v {list(vshape)} must be [rows, key heads, '
                          '64 or 128] alike')
     cache, sizes = _check_cache(k_pages, v_pages, k_exp, v_exp, table, heads, d, dev)
-    # (V and its exponents have K's strides)
+    # (V and its exponents have K's strides; K may be V where their new rows are one too)
+    alike = ka == va or k_pages.shape[0] == 0
     shared = any(n > 1 and s == 0 for n, s in zip(k_pages.shape, k_pages.stride()))
-    shared |= k_pages.data_ptr() == v_pages.data_ptr() and k_pages.shape[0] > 0
+    shared |= not alike and k_pages.data_ptr() == v_pages.data_ptr()
     if k_exp is not None and not shared:
         shared = (any(n > 1 and s == 0 for n, s in zip(k_exp.shape, k_exp.stride()))
-                  or (k_exp.data_ptr() == v_exp.data_ptr() and k_exp.shape[0] > 0))
+                  or (not alike and k_exp.data_ptr() == v_exp.data_ptr()))
     if shared:
         raise ValueError('cache_append_ needs a cache whose rows and exponents do not share memory')
     n = table.shape[0]

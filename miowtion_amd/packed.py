@@ -143,8 +143,8 @@ def cache_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, cu: torch
     cache are left out; every other row of the cache stays as it was. Two rows
     written to one place by one call (a page that two sequences share where both
     write): which of them the cache then holds is undefined. A cache that holds
-    two of its rows, or their exponents, in one place by a stride of 0, or K where
-    it holds V, is refused.
+    two of its rows, or their exponents, in one place by a stride of 0, is refused,
+    and so is one that holds K where it holds V, unless k and v are one tensor too.
 
     cu int32 [B + 1], table int32 [B, pages of a sequence], start int32 [B].
     """

@@ -106,6 +106,20 @@ def test_exponents_that_share_memory_are_not_written():
     assert torch.equal(got[:, 0], want[:, 0])
 
 
+@pytest.mark.parametrize('dtype', [BF16, torch.float8_e4m3fn], ids=['bf16', 'e4m3'])
+def test_one_cache_for_keys_and_values(dtype):
+    """Rows that are both: written where k and v are one tensor too."""
+    cache, table, lengths, k, v, start, cu = _cache(dtype)
+    kernels.cache_append_(cache, k, k, cu, table, start)
+    other = kernels.paged_cache(8, 16, 2, 64, dtype)
+    one = other._replace(v=other.k, v_exp=other.k_exp)
+    kernels.cache_append_(one, k, k, cu, table, start)
+    for a, b in zip(one, cache):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    with pytest.raises(ValueError, match='share memory'):
+        kernels.cache_append_(one, k, v, cu, table, start)
+
+
 def test_calls_on_two_streams_at_once():
     lens = [700, 300]
     cases = [_inputs(lens, lens, 8, 2, 128, seed=s) for s in range(4)]

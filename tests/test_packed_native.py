@@ -237,6 +237,7 @@ def test_caches_that_share_memory_are_not_written():
     k, cu = _cpu(4, 2, 64), _cpu(2, dtype=torch.int32)
     table, one = _cpu(1, 2, dtype=torch.int32), _cpu(1, dtype=torch.int32)
     append = ops_packed.cache_append_._fn  # what runs behind the refusal of CPU tensors
+    v = _cpu(4, 2, 64)
     for cache in _shared_caches():
         with pytest.raises(ValueError, match='share memory'):
-            append(*cache, k, k, cu, table, one)
+            append(*cache, k, v, cu, table, one)
