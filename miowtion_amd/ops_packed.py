@@ -220,6 +220,12 @@ def _check_cache(k_pages, v_pages, k_exp, v_exp, table, heads, d, dev):
             [shape[0], shape[1], table.data_ptr(), table.stride(0), table.shape[1]])
 
 
+def _folded(t: torch.Tensor) -> bool:
+    """Whether a stride of 0 holds several of t's values in one place."""
+    strides = t.stride()
+    return 0 in strides and any(n > 1 and s == 0 for n, s in zip(t.shape, strides))
+
+
 @_custom_op('veda::cache_append_', mutates_args=('k_pages', 'v_pages', 'k_exp', 'v_exp'))
 def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exp: torch.Tensor | None,
                   v_exp: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor,
@@ -232,12 +238,9 @@ def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k_exp: torch.Ten
                          '64 or 128] alike')
     cache, sizes = _check_cache(k_pages, v_pages, k_exp, v_exp, table, heads, d, dev)
     # (V and its exponents have K's strides; K may be V where their new rows are one too)
-    alike = ka == va or k_pages.shape[0] == 0
-    shared = any(n > 1 and s == 0 for n, s in zip(k_pages.shape, k_pages.stride()))
-    shared |= not alike and k_pages.data_ptr() == v_pages.data_ptr()
-    if k_exp is not None and not shared:
-        shared = (any(n > 1 and s == 0 for n, s in zip(k_exp.shape, k_exp.stride()))
-                  or (not alike and k_exp.data_ptr() == v_exp.data_ptr()))
+    shared = _folded(k_pages) or (k_exp is not None and _folded(k_exp))
+    if cache[0] == cache[1] or (k_exp is not None and cache[6] == cache[7]):
+        shared |= ka != va and k_pages.shape[0] > 0
     if shared:
         raise ValueError('cache_append_ needs a cache whose rows and exponents do not share memory')
     n = table.shape[0]
