@@ -681,6 +681,68 @@ int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                    float* lse, void* workspace, int64_t workspace_bytes,
                    void* stream);
 
+/*
+ * Norms of query and key heads, and their rotation by position:
+ *   z = x r w,  r = (mean(x^2) + eps)^-1/2  (eps < 0: z = x, w unused)
+ *   (y_a, y_b) = (z_a cos f - z_b sin f, z_b cos f + z_a sin f),
+ *   f = 2 pi turns[pair] * positions[row, axes[pair]]
+ * for the n_pairs pairs (a, b) = (j, j + n_pairs), or (2 j, 2 j + 1) with
+ * `adjacent`; other dims stay as they are. n_pairs 0: no rotation; not adjacent,
+ * a multiple of 8. eps at least 1e-30.
+ * q, k: bf16 [rows, q_heads | k_heads, D], D 64 or 128, strides (stride_s,
+ * stride_h, 1), every row 16-byte aligned; either may have no heads. positions:
+ * strides (stride_t, stride_a), kind 0 int32, 1 int64, 2 fp32. turns: fp64
+ * [n_pairs], axes: int32 [n_pairs] (taken as within [0, n_axes)). Weights [D],
+ * bf16 or fp32, NULL for ones. q_out, k_out: bf16 [rows, heads, D] contiguous.
+ */
+int veda_norm_rotate(const void* q, int64_t q_stride_s, int64_t q_stride_h,
+                     int64_t q_heads, const void* k, int64_t k_stride_s,
+                     int64_t k_stride_h, int64_t k_heads, int64_t rows,
+                     int64_t head_dim, const void* positions, int64_t kind,
+                     int64_t stride_t, int64_t stride_a, const double* turns,
+                     const int32_t* axes, int64_t n_pairs, int64_t n_axes,
+                     int adjacent, const void* q_weight, int q_weight_bf16,
+                     const void* k_weight, int k_weight_bf16, float eps,
+                     void* q_out, void* k_out, void* stream);
+
+/*
+ * Gradients of veda_norm_rotate: dz = dy rotated back, dw = sum dz x r,
+ * dx = r (g - x r mean(g x r)) with g = dz w. dq_out, dk_out: the gradients of
+ * its results, bf16, strided as q and k are. dq, dk: bf16 [rows, heads, D]
+ * contiguous. dq_weight, dk_weight: [D] of the weights' types, or NULL; with
+ * either, workspace holds 1,024 * 2 * D floats, 16-byte aligned. Sums are taken in
+ * an order that the sizes set: the same bits on every call.
+ */
+int veda_norm_rotate_bwd(
+    const void* q, int64_t q_stride_s, int64_t q_stride_h, const void* dq_out,
+    int64_t dq_stride_s, int64_t dq_stride_h, int64_t q_heads, const void* k,
+    int64_t k_stride_s, int64_t k_stride_h, const void* dk_out, int64_t dk_stride_s,
+    int64_t dk_stride_h, int64_t k_heads, int64_t rows, int64_t head_dim,
+    const void* positions, int64_t kind, int64_t stride_t, int64_t stride_a,
+    const double* turns, const int32_t* axes, int64_t n_pairs, int64_t n_axes,
+    int adjacent, const void* q_weight, int q_weight_bf16, const void* k_weight,
+    int k_weight_bf16, float eps, void* dq, void* dk, void* dq_weight, void* dk_weight,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * veda_norm_rotate of q and k, and veda_cache_append of the k that it gives and
+ * of v, in one launch; e4m3 keys are rounded from 32 bits once. positions NULL:
+ * a row's position in its sequence (start[b] + i) on every axis. q_out: rows of
+ * no sequence are zeros.
+ */
+int veda_cache_append_rotated(
+    const void* q, int64_t q_stride_s, int64_t q_stride_h, int64_t q_heads, const void* k,
+    int64_t k_stride_s, int64_t k_stride_h, const void* v, int64_t v_stride_s,
+    int64_t v_stride_h, int64_t rows, int64_t n_kv_heads, int64_t head_dim,
+    const int32_t* cu, const int32_t* start, int64_t n_seq, void* k_pages, void* v_pages,
+    int64_t stride_p, int64_t stride_s, int64_t stride_h, int e4m3, uint8_t* k_exp,
+    uint8_t* v_exp, int64_t exp_stride_p, int64_t exp_stride_s, int64_t exp_stride_h,
+    int64_t n_pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
+    const void* positions, int64_t kind, int64_t stride_t, int64_t stride_a,
+    const double* turns, const int32_t* axes, int64_t n_pairs, int64_t n_axes, int adjacent,
+    const void* q_weight, int q_weight_bf16, const void* k_weight, int k_weight_bf16,
+    float eps, void* q_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

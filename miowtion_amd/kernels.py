@@ -13,7 +13,8 @@ signatures:
 
 and, beside dense_attention, those of packed sequences and the paged cache
 (packed_attention, cache_append_, cache_gather, paged_attention; no reference
-counterpart, `miowtion_amd.packed`).
+counterpart, `miowtion_amd.packed`), and the norms and rotations of q and k before
+them (norm_rotate, cache_append_rotated_; `miowtion_amd.rotary`).
 
 All run on the GPU through `miowtion_amd.ops`; CPU tensors raise
 NotImplementedError (no fallback, never a silent dense path).
@@ -27,6 +28,7 @@ from miowtion_amd import ops
 from miowtion_amd import tiling
 from miowtion_amd.packed import (PagedCache, cache_append_, cache_gather, packed_attention,  # noqa: F401
                                  paged_attention, paged_cache)
+from miowtion_amd.rotary import Rotary, cache_append_rotated_, norm_rotate, rotary  # noqa: F401
 
 SECOND_RAW = 'raw'
 SECOND_CENTRAL = 'central'
