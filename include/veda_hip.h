@@ -682,6 +682,25 @@ int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
                    void* stream);
 
 /*
+ * Attention of a chunk of new tokens of every sequence over its cache: as
+ * veda_packed_fwd with cu for cu_q and, for keys and values of sequence b, its first
+ * lengths[b] positions (clamped to the table's width; positions of no row draw no
+ * weight). n_split (1 .. 64): workgroups that share the keys of 128 rows; above 1,
+ * workspace holds n_split * q_rows * n_heads * (D + 2) floats, 16-byte aligned.
+ */
+int veda_chunk_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h, int64_t q_rows,
+                   int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                   const int32_t* cu, int64_t n_seq, const void* k_pages,
+                   const void* v_pages, int64_t stride_p, int64_t stride_s,
+                   int64_t stride_h, int e4m3, const uint8_t* k_exp,
+                   const uint8_t* v_exp, int64_t exp_stride_p, int64_t exp_stride_s,
+                   int64_t exp_stride_h, int64_t n_pages, int64_t page,
+                   const int32_t* table, int64_t table_ld, int64_t width,
+                   const int32_t* lengths, int causal, float scale, int64_t n_split,
+                   void* out, int64_t o_stride_s, int64_t o_stride_h, float* lse,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Norms of query and key heads, and their rotation by position:
  *   z = x r w,  r = (mean(x^2) + eps)^-1/2  (eps < 0: z = x, w unused)
  *   (y_a, y_b) = (z_a cos f - z_b sin f, z_b cos f + z_a sin f),

@@ -30,11 +30,11 @@ FLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}',
          f'-I{ROOT / "include"}']
 
 
-# Per-source extra flags. attention.hip, heat.hip, packed.hip, paged.hip: MFMA
+# Per-source extra flags. attention, chunk, heat, packed and paged.hip: MFMA
 # results in VGPRs (the softmax / heat reads every score; the default AGPR form
 # costs a copy per score).
 EXTRA = {name: ['-mllvm', '-amdgpu-mfma-vgpr-form']
-         for name in ('attention.hip', 'heat.hip', 'packed.hip', 'paged.hip')}
+         for name in ('attention.hip', 'chunk.hip', 'heat.hip', 'packed.hip', 'paged.hip')}
 
 
 def sources() -> list[pathlib.Path]:

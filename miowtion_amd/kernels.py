@@ -12,8 +12,8 @@ signatures:
   teacher_heat                    miowtion/kernels/block_heat_triton.py:141-173
 
 and, beside dense_attention, those of packed sequences and the paged cache
-(packed_attention, cache_append_, cache_gather, paged_attention; no reference
-counterpart, `miowtion_amd.packed`), and the norms and rotations of q and k before
+(packed_attention, cache_append_, cache_gather, paged_attention,
+paged_chunk_attention; no reference counterpart, `miowtion_amd.packed`), and the norms and rotations of q and k before
 them (norm_rotate, cache_append_rotated_; `miowtion_amd.rotary`).
 
 All run on the GPU through `miowtion_amd.ops`; CPU tensors raise
@@ -27,7 +27,7 @@ import torch
 from miowtion_amd import ops
 from miowtion_amd import tiling
 from miowtion_amd.packed import (PagedCache, cache_append_, cache_gather, packed_attention,  # noqa: F401
-                                 paged_attention, paged_cache)
+                                 paged_attention, paged_cache, paged_chunk_attention)
 from miowtion_amd.rotary import Rotary, cache_append_rotated_, norm_rotate, rotary  # noqa: F401
 
 SECOND_RAW = 'raw'

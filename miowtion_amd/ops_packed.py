@@ -326,3 +326,35 @@ def paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 def _(q, k_pages, v_pages, k_exp, v_exp, table, lengths, scale, return_lse):
     out = q.new_empty(q.shape)
     return [out, q.new_empty(q.shape[:2], dtype=torch.float32)] if return_lse else [out]
+
+
+@_custom_op('veda::chunk_fwd', mutates_args=())
+def chunk_fwd(q: torch.Tensor, cu: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+              k_exp: torch.Tensor | None, v_exp: torch.Tensor | None, table: torch.Tensor,
+              lengths: torch.Tensor, causal: bool, scale: float, return_lse: bool) -> list[torch.Tensor]:
+    """[out] or [out, lse]: out [T, H, D] bf16, lse [T, H] fp32."""
+    dev = q.get_device()
+    (rows, heads, d), *qa = _rows('q', q, dev)
+    kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
+    if d not in HEAD_DIMS or kv == 0 or heads == 0 or heads % kv:
+        raise ValueError(f'q {[rows, heads, d]} does not fit a cache of {kv} key heads: head_dim 64 or '
+                         '128, query heads a multiple of the key heads')
+    cache, sizes = _check_cache(k_pages, v_pages, k_exp, v_exp, table, kv, d, dev)
+    n = table.shape[0]
+    n_split = _key_splits(rows, n * table.shape[1] * k_pages.shape[1], n, heads, kv)
+    out = q.new_empty((rows, heads, d))
+    lse = q.new_empty((rows, heads), dtype=_F32) if return_lse else None
+    work, nbytes = None, 0
+    if n_split > 1:
+        nbytes = 4 * n_split * rows * heads * (d + 2)
+        work = q.new_empty(nbytes // 4, dtype=_F32)
+    _launch('veda_chunk_fwd', dev, *qa, rows, heads, kv, d, _ints('cu', cu, n + 1, dev), n, *cache, *sizes,
+            _ints('lengths', lengths, n, dev), causal, scale, n_split, out.data_ptr(), heads * d, d,
+            lse.data_ptr() if return_lse else None, None if work is None else work.data_ptr(), nbytes)
+    return [out, lse] if return_lse else [out]
+
+
+@chunk_fwd.register_fake
+def _(q, cu, k_pages, v_pages, k_exp, v_exp, table, lengths, causal, scale, return_lse):
+    out = q.new_empty(q.shape)
+    return [out, q.new_empty(q.shape[:2], dtype=torch.float32)] if return_lse else [out]

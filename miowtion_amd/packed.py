@@ -188,3 +188,38 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, table: torch.Tensor, len
     res = ops_packed.paged_fwd(q, cache.k, cache.v, cache.k_exp, cache.v_exp, table, lengths,
                                _scale(scale, q.shape[-1]), return_lse)
     return (res[0], res[1]) if return_lse else res[0]
+
+
+def paged_chunk_attention(q: torch.Tensor, cu: torch.Tensor, cache: PagedCache, table: torch.Tensor,
+                          lengths: torch.Tensor, causal: bool = True, scale: float | None = None,
+                          return_lse: bool = False):
+    """Attention of the last tokens of every sequence over its cached positions, read
+    from the pages as they lie: what packed_attention gives with the k and v of
+    cache_gather, without the copy.
+
+    Args:
+        q: [T, H, D] bf16, D 64 or 128, H a multiple of the cache's key heads; rows in any
+            strides on 16-byte boundaries.
+        cu: int32 [B + 1], ascending: sequence b has the rows cu[b] .. cu[b + 1] - 1 of q,
+            as many as it likes, none too. Offsets outside the rows are clamped.
+        cache: holds the new tokens' own rows too (append them first).
+        table: int32 [B, pages of a sequence], rows in any stride. Its width is what the
+            host knows of the lengths, and sets how many workgroups may share a sequence.
+        lengths: int32 [B]: the keys of sequence b are its positions 0 .. lengths[b] - 1
+            (at most the table's width). Positions in a page outside the cache draw no
+            weight.
+        causal: query i of n_q sees the keys up to i + lengths[b] - n_q; else all.
+        scale: of the scores; None: D ** -0.5. Positive.
+        return_lse: also return the [T, H] fp32 natural-log LSE.
+
+    Returns:
+        out [T, H, D] bf16, or (out, lse). Rows that see no key, and rows of no sequence,
+        have out 0 and lse -inf. A key that a row does not see does not touch its out,
+        whatever it holds. The same bits on every call with these shapes. Rounded as
+        packed_attention's.
+
+    Without gradients, as the cache has none.
+    """
+    res = ops_packed.chunk_fwd(q, cu, cache.k, cache.v, cache.k_exp, cache.v_exp, table, lengths, causal,
+                               _scale(scale, q.shape[-1]), return_lse)
+    return (res[0], res[1]) if return_lse else res[0]
