@@ -685,8 +685,10 @@ int veda_paged_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h,
  * Attention of a chunk of new tokens of every sequence over its cache: as
  * veda_packed_fwd with cu for cu_q and, for keys and values of sequence b, its first
  * lengths[b] positions (clamped to the table's width; positions of no row draw no
- * weight). n_split (1 .. 64): workgroups that share the keys of 128 rows; above 1,
- * workspace holds n_split * q_rows * n_heads * (D + 2) floats, 16-byte aligned.
+ * weight). n_split (1 .. 64): workgroups that may share the keys of 128 rows; above 1,
+ * workspace holds q_rows * n_heads * (n_split * (D + 2) + 1) floats, 16-byte aligned.
+ * units (1 .. 2^20): workgroups for each key head that keys are shared among, so far
+ * as n_split lets them (up to 126 sequences; beyond, each shares its own).
  */
 int veda_chunk_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h, int64_t q_rows,
                    int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
@@ -697,8 +699,8 @@ int veda_chunk_fwd(const void* q, int64_t q_stride_s, int64_t q_stride_h, int64_
                    int64_t exp_stride_h, int64_t n_pages, int64_t page,
                    const int32_t* table, int64_t table_ld, int64_t width,
                    const int32_t* lengths, int causal, float scale, int64_t n_split,
-                   void* out, int64_t o_stride_s, int64_t o_stride_h, float* lse,
-                   void* workspace, int64_t workspace_bytes, void* stream);
+                   int64_t units, void* out, int64_t o_stride_s, int64_t o_stride_h,
+                   float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Norms of query and key heads, and their rotation by position:

@@ -82,7 +82,7 @@ SIGNATURES: dict[str, list] = {
     'veda_paged_fwd': [_P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I, _I, _C, _P, _P, _I, _I, _I, _I,
                        _I, _P, _I, _I, _P, _F, _I, _P, _I, _I, _P, _P, _I, _P],
     'veda_chunk_fwd': [_P, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _C, _P, _P, _I, _I, _I,
-                       _I, _I, _P, _I, _I, _P, _C, _F, _I, _P, _I, _I, _P, _P, _I, _P],
+                       _I, _I, _P, _I, _I, _P, _C, _F, _I, _I, _P, _I, _I, _P, _P, _I, _P],
     'veda_norm_rotate': [_P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P, _I, _I, _C,
                          _P, _C, _P, _C, _F, _P, _P, _P],
     'veda_norm_rotate_bwd': [_P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _I,

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_fwd_kernel(FwdArgs p) {
     stage<D, false, kSmSecond, true>(s0, cur, f, c, sb, sb, pb, pa, w, NoHook{});
     stage<D, false, kNoSm, true>(s0, cur + kSub, f, c, sa, sb, pa, pb, w, NoHook{});
   }
-  leave_rows<D>(p, w, sp, split, head, r0, rows, limit, wave, lane, s0,
+  leave_rows<D>(p, w, sp, split, p.n_split, head, r0, rows, limit, wave, lane, s0,
                 [&](int64_t tok, int64_t hd, int lim, float mu, float inv, float* part) {
                   redo_row<D>(p.q + tok * p.qs + hd * p.qh, kbase, vbase, p.ks, p.vs, lim, c, mu, inv,
                               p.out + tok * p.os + hd * p.oh, part, lane);

@@ -108,6 +108,23 @@ __device__ __forceinline__ bf16x8 vt_frag(const lds_u8* vb, const Frags<D>& f, i
   return join_tr(a, a + 8 * Tile<D>::kPitch);
 }
 
+// The end of a sub-block's softmax: its sums l4 to the row's, or its probabilities again
+// against a raised reference.
+template <int D, int SM>
+__device__ __forceinline__ void take_sums(const float (&l4)[4], const f32x16& sp, float c, u32x4 (&pn)[2],
+                                          Wave<D>& w) {
+  const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+  if (__builtin_expect(!(w.have_ref && __ballot(sum < kLazyLimit) == ~0ull), 0)) {
+    if (SM == kSmSecond) w.l_run += w.first_sum;
+    w.first_sum = 0.f;
+    raise_reference<D>(sp, c, pn, w);
+  } else if (SM == kSmFirst) {
+    w.first_sum = sum;
+  } else {
+    w.l_run += w.first_sum + sum;
+  }
+}
+
 template <int D, bool QK, int SM, bool PV, int NEXT = kNoNext, typename Hook>
 __device__ __forceinline__ void stage(const lds_u8* kb, const lds_u8* vb, const Frags<D>& f, float c,
                                       f32x16& sn, const f32x16& sp, u32x4 (&pn)[2],
@@ -158,28 +175,17 @@ __device__ __forceinline__ void stage(const lds_u8* kb, const lds_u8* vb, const 
     __builtin_amdgcn_sched_barrier(0);
   }
   w.alpha = 1.f;
-  if (SM != kNoSm) {
-    const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-    if (__builtin_expect(!(w.have_ref && __ballot(sum < kLazyLimit) == ~0ull), 0)) {
-      if (SM == kSmSecond) w.l_run += w.first_sum;
-      w.first_sum = 0.f;
-      raise_reference<D>(sp, c, pn, w);
-    } else if (SM == kSmFirst) {
-      w.first_sum = sum;
-    } else {
-      w.l_run += w.first_sum + sum;
-    }
-  }
+  if (SM != kNoSm) take_sums<D, SM>(l4, sp, c, pn, w);
 }
 
-// A wave's rows once the walk is done: out and lse, or, where the keys are split, this
-// split's O, reference (log2) and sum of weights; O leaves as whole rows, by way of
+// A wave's rows once the walk is done: out and lse, or, of one of several `splits` of the
+// keys, the split's O, reference (log2) and sum of weights; O leaves as whole rows, by way of
 // the wave's part of the ring. again(token, head, limit, reference, 1 / l, part):
 // forms a row anew whose O came out with a NaN though its sum of weights has none.
 // limit: the keys that the lane's row sees.
 template <int D, typename Args, typename Again>
 __device__ __forceinline__ void leave_rows(const Args& p, const Wave<D>& w, const Span& sp, int split,
-                                           int head, int r0, int rows, int limit, int wave, int lane,
+                                           int splits, int head, int r0, int rows, int limit, int wave, int lane,
                                            lds_u8* s0, Again again) {
   using T = Tile<D>;
   const int li = lane & 31, hi = lane >> 5;
@@ -192,7 +198,7 @@ __device__ __forceinline__ void leave_rows(const Args& p, const Wave<D>& w, cons
   const float l = half_swap_sum(l_run);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;
-  if (p.lse != nullptr && hi == 0 && real && p.n_split == 1)
+  if (p.lse != nullptr && hi == 0 && real && splits == 1)
     p.lse[token * n_heads + qhead] = l == 0.f ? -INFINITY : (m_run + __log2f(l)) * kLn2;
   bool bad = false;
 #pragma unroll
@@ -210,10 +216,10 @@ __device__ __forceinline__ void leave_rows(const Args& p, const Wave<D>& w, cons
       const int64_t tok = sp.q0 + row / p.pk.group, hd = (int64_t)head * p.pk.group + row % p.pk.group;
       const float m = __shfl(m_run, rr);
       again(tok, hd, __shfl(limit, rr), m == -INFINITY ? 0.f : m, __shfl(inv, rr),
-            p.n_split > 1 ? p.part + (split * all_rows + tok * n_heads + hd) * D : nullptr);
+            splits > 1 ? p.part + (split * all_rows + tok * n_heads + hd) * D : nullptr);
     }
   };
-  if (p.n_split > 1) {
+  if (splits > 1) {
     if (real) {
       const int64_t at = split * all_rows + token * n_heads + qhead;
       if (hi == 0)

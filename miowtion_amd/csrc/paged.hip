@@ -139,20 +139,6 @@ struct TokenArgs {
   float* part;  // [B, H, n_split, D + 4]: O, then the reference (log2) and the sum
 };
 
-template <int D>
-__device__ __forceinline__ int swz_v(int r) {
-  return D == 128 ? ((r & 3) << 2) | ((((r >> 2) ^ (r >> 3)) & 1) << 1) | ((r >> 3) & 1)
-                  : (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
-}
-
-// Maximum and sum over the four lane groups of a query head (lanes n + 16 g).
-template <bool MAX>
-__device__ __forceinline__ float over_groups(float v) {
-  const float w = __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401F));
-  v = MAX ? fmaxf(v, w) : v + w;
-  return MAX ? half_swap_max(v) : half_swap_sum(v);
-}
-
 __device__ __forceinline__ int length_of(const TokenArgs& p, int b) {
   return min(max(p.lengths[b], 0), p.tab.width << p.tab.shift);
 }

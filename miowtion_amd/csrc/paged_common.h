@@ -149,6 +149,22 @@ __device__ __forceinline__ u32x2 encode8(const float (&x)[8], uint32_t& byte) {
   return w;
 }
 
+// V rows of a wave's own in LDS that are read transposed by 16x16 products: the chunk's
+// place is xor'ed with this.
+template <int D>
+__device__ __forceinline__ int swz_v(int r) {
+  return D == 128 ? ((r & 3) << 2) | ((((r >> 2) ^ (r >> 3)) & 1) << 1) | ((r >> 3) & 1)
+                  : (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
+}
+
+// Maximum and sum over the four lane groups of a query head (lanes n + 16 g).
+template <bool MAX>
+__device__ __forceinline__ float over_groups(float v) {
+  const float w = __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401F));
+  v = MAX ? fmaxf(v, w) : v + w;
+  return MAX ? half_swap_max(v) : half_swap_sum(v);
+}
+
 inline bool whole(const void* p, int64_t mult, int64_t a, int64_t b, int64_t c) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && a % mult == 0 && b % mult == 0 && c % mult == 0;
 }

@@ -11,6 +11,8 @@ refuses them with the same ValueError.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from miowtion_amd import _native
@@ -18,6 +20,7 @@ from miowtion_amd.ops import TILE, _custom_op, _p, _raw_stream
 
 HEAD_DIMS = (64, 128)
 PAGES = (16, 32, 64, 128, 256)
+_CHUNK_WORK = 1 << 27
 _BF16, _F32, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
 # absent from a torch built without a GPU, where no op gets as far as a launch
 _current_device = getattr(torch._C, '_cuda_getDevice', None)
@@ -328,6 +331,19 @@ def _(q, k_pages, v_pages, k_exp, v_exp, table, lengths, scale, return_lse):
     return [out, q.new_empty(q.shape[:2], dtype=torch.float32)] if return_lse else [out]
 
 
+def _chunk_splits(rows: int, heads: int, kv_heads: int, d: int, n_seq: int, capacity: int) -> tuple[int, int]:
+    """(splits of a row's keys at most, workgroups wanted for each key head) of chunk_fwd. How
+    many splits a sequence gets is up to its length, which is on the GPU."""
+    resident = max((512 if d == 128 else 768) // kv_heads, 1)
+    tiles = rows * heads // kv_heads // TILE + min(n_seq, rows)
+    units = min(int(math.sqrt(tiles * capacity * resident / 1024)), 2 * resident) + 1
+    if n_seq <= 126:
+        most = min(-(-capacity // 256), _CHUNK_WORK // max(4 * rows * heads * (d + 2), 1), 64)
+    else:
+        most = min(-(-capacity // 256), -(-512 // (n_seq * kv_heads)))
+    return max(most, 1), units
+
+
 @_custom_op('veda::chunk_fwd', mutates_args=())
 def chunk_fwd(q: torch.Tensor, cu: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
               k_exp: torch.Tensor | None, v_exp: torch.Tensor | None, table: torch.Tensor,
@@ -341,16 +357,16 @@ def chunk_fwd(q: torch.Tensor, cu: torch.Tensor, k_pages: torch.Tensor, v_pages:
                          '128, query heads a multiple of the key heads')
     cache, sizes = _check_cache(k_pages, v_pages, k_exp, v_exp, table, kv, d, dev)
     n = table.shape[0]
-    n_split = _key_splits(rows, n * table.shape[1] * k_pages.shape[1], n, heads, kv)
+    n_split, units = _chunk_splits(rows, heads, kv, d, n, table.shape[1] * k_pages.shape[1])
     out = q.new_empty((rows, heads, d))
     lse = q.new_empty((rows, heads), dtype=_F32) if return_lse else None
     work, nbytes = None, 0
     if n_split > 1:
-        nbytes = 4 * n_split * rows * heads * (d + 2)
+        nbytes = 4 * rows * heads * (n_split * (d + 2) + 1)
         work = q.new_empty(nbytes // 4, dtype=_F32)
     _launch('veda_chunk_fwd', dev, *qa, rows, heads, kv, d, _ints('cu', cu, n + 1, dev), n, *cache, *sizes,
-            _ints('lengths', lengths, n, dev), causal, scale, n_split, out.data_ptr(), heads * d, d,
-            lse.data_ptr() if return_lse else None, None if work is None else work.data_ptr(), nbytes)
+            _ints('lengths', lengths, n, dev), causal, scale, n_split, units, out.data_ptr(),
+            heads * d, d, lse.data_ptr() if return_lse else None, None if work is None else work.data_ptr(), nbytes)
     return [out, lse] if return_lse else [out]
 
 
