@@ -405,6 +405,7 @@ __device__ __forceinline__ void stage8(const lds_u8* kb, const lds_u8* ke, const
     const int i = j / kEvery;
     if (QK && j % (8 / kTerms) == 0) {
       const int term = j / (8 / kTerms);
+      if (term > 0) asm volatile("" : "+v"(sn));  // formed here, not sunk to its use
       if (D == 128 && term == 0) kf[D / 64 - 1] = code_frag(kb, cf.k[D / 32 - 2], cf.k[D / 32 - 1]);
       if (term == 0) sn = code_product<D, 0>(kf[0], k_scale, q, sn);
       if (term == 1) sn = code_product<D, 1>(kf[0], k_scale, q, sn);
@@ -425,12 +426,13 @@ __device__ __forceinline__ void stage8(const lds_u8* kb, const lds_u8* ke, const
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+  if (QK) asm volatile("" : "+v"(sn));
   w.alpha = 1.f;
   if (SM != kNoSm) take_sums<D, SM>(l4, sp, c, pn, w);
 }
 
 // ---------------------------------------------------------------------------
-// A sequence of at most 32 rows (few new tokens): each wave takes tiles of 32 keys of its
+// A sequence of at most 32 rows (few new tokens), 16 NB at most: each wave takes tiles of 32 keys of its
 // own, every fourth of the unit's, for all rows, and nothing waits for another wave
 // until the end, as in the attention of one token (paged.hip has the layout of its
 // 16x16 products): K goes from memory straight into the operand, V through the wave's
@@ -438,10 +440,9 @@ __device__ __forceinline__ void stage8(const lds_u8* kb, const lds_u8* ke, const
 // one wave would have all the work of such a tile and three none (eight sequences of
 // 2,000 to 8,192, 16 rows: @FEW@).
 
-template <int D, bool F8>
+template <int D, bool F8, int NB>
 __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, const Queries& of, int head, int rows,
                                          int from, int n_steps, int last, int wave, int lane, lds_u8* s0) {
-  constexpr int kNB = 2;                      // blocks of 16 rows
   constexpr int kPitch = 2 * D;               // a V row in LDS, bf16
   constexpr int kTileBytes = 32 * kPitch;
   constexpr int kPer = F8 ? 16 : 8;           // elements of a 16-byte load
@@ -453,7 +454,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
   constexpr int kVLoads = 32 / kVRows;
   constexpr int kDB = D / 16;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  __shared__ float red_m[4][16 * kNB], red_l[4][16 * kNB];
+  __shared__ float red_m[4][16 * NB], red_l[4][16 * NB];
   const Span& sp = unit.sp;
   const int n = lane & 15, g = lane >> 4, b = sp.seq - 1;
   const int begin = 64 * from, end = min(64 * (from + n_steps), last);
@@ -461,10 +462,10 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
   const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;
   const int64_t row0 = sp.q0 * n_heads + (int64_t)head * p.pk.group;
   // Q: row 16 nb + n, in the order of the K loads' elements; the keys that it sees
-  bf16x8 qf[kNB][kSteps];
-  int lim[kNB];
+  bf16x8 qf[NB][kSteps];
+  int lim[NB];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
     const int r = min(16 * nb + n, rows - 1);
     lim[nb] = min(seen(p, sp, of.query(r)), end);
     const uint16_t* qrow = p.q + (sp.q0 + of.query(r)) * p.qs + ((int64_t)head * p.pk.group + of.head(r)) * p.qh;
@@ -518,10 +519,10 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
   // transposed reads: rows 4 g + n / 4 (and 16 on), column block db at xor 32 db
   const int tr_row = 4 * g + (n >> 2);
   const uint32_t tr = (uint32_t)(tr_row * kPitch + ((((n >> 1) & 1) ^ swz_v<D>(tr_row)) << 4) + 8 * (n & 1));
-  f32x4 o[kNB][kDB];
-  float m_run[kNB], l_run[kNB];
+  f32x4 o[NB][kDB];
+  float m_run[NB], l_run[NB];
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
     for (int db = 0; db < kDB; ++db) o[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     m_run[nb] = -INFINITY;
@@ -544,7 +545,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
 #pragma unroll
       for (int i = 0; i < 2; ++i) next[i] = __builtin_amdgcn_readlane(pages[i], tile + 1 - window);
     }
-    f32x4 s[kNB][2];
+    f32x4 s[NB][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       u32x4 a[kSteps];
@@ -554,7 +555,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
         else a[t % kSteps] = kreg[i][t];
       }
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
+      for (int nb = 0; nb < NB; ++nb) {
         s[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < kSteps; ++t)
@@ -566,10 +567,10 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
     // rows of V that some row sees
     const int live[2] = {now[0] >= 0 ? end - j : 0, now[1] >= 0 ? end - j - 16 : 0};
     const bool masked = j + 32 > see_all || now[0] < 0 || now[1] < 0;
-    u32x4 pb[kNB];
-    float alpha[kNB];
+    u32x4 pb[NB];
+    float alpha[NB];
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
+    for (int nb = 0; nb < NB; ++nb) {
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -622,7 +623,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
       const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(x + 16 * kPitch));
       const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nb][db][e] *= alpha[nb];
         o[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, as_bf16x8(pb[nb]), o[nb][db], 0, 0, 0);
@@ -637,7 +638,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
   // The waves' sums, at the largest of their references, by way of LDS: O^T of lane
   // (n, g) is head-dims 16 db + 4 g .. + 3 of row 16 nb + n.
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
     l_run[nb] = over_groups<false>(l_run[nb]);
     if (g == 0) {
       red_m[wave][16 * nb + n] = m_run[nb];
@@ -646,7 +647,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
   }
   const int tid = 64 * wave + lane, qn = tid >> 4;
 #pragma unroll
-  for (int nb = 0; nb < kNB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
     __syncthreads();
     {
       float m = -INFINITY;
@@ -761,10 +762,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkA
   };
   const int from = begins(unit.split);
   const int n_steps = begins(unit.split + 1) - from;
-  if (rows <= 32) {
-    few_rows<D, F8>(p, unit, of, head, rows, from, n_steps, last, wave, lane, (lds_u8*)ring);
-    return;
-  }
+  if (rows <= 16) return few_rows<D, F8, 1>(p, unit, of, head, rows, from, n_steps, last, wave, lane, (lds_u8*)ring);
+  if (rows <= 32) return few_rows<D, F8, 2>(p, unit, of, head, rows, from, n_steps, last, wave, lane, (lds_u8*)ring);
   const int end = 64 * n_steps;
   const int limit = min(max((real ? seen(p, sp, of.query(r - r0)) : last) - 64 * from, 0), end);
   const int n_plain = min(max(seen(p, sp, of.first) - 64 * from, 0), end) >> 6;  // seen whole by every row
