@@ -731,7 +731,7 @@ int veda_norm_rotate(const void* q, int64_t q_stride_s, int64_t q_stride_h,
  * dx = r (g - x r mean(g x r)) with g = dz w. dq_out, dk_out: the gradients of
  * its results, bf16, strided as q and k are. dq, dk: bf16 [rows, heads, D]
  * contiguous. dq_weight, dk_weight: [D] of the weights' types, or NULL; with
- * either, workspace holds 1,024 * 2 * D floats, 16-byte aligned. Sums are taken in
+ * either, workspace holds 768 * 2 * D floats, 16-byte aligned. Sums are taken in
  * an order that the sizes set: the same bits on every call.
  */
 int veda_norm_rotate_bwd(

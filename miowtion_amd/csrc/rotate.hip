@@ -43,6 +43,24 @@ struct Heads {
   int32_t n;
 };
 
+// How rows are moved: past the caches where they would not stay there anyway. Rows that
+// are written leave the GPU's L2 from some 32 MB on (a preview's 38 MB of q and k: 16.5 us
+// kept, 15.6 past it; 153 MB 60 and 48), rows that are read all caches from 256 MB on (1.4
+// GB: 516 us kept, 494 past them; 153 MB 48 and 58, for what a projection has just written is
+// still there).
+enum { kKept = 0, kStoresPast = 1, kAllPast = 2 };
+
+template <int MOVE>
+__device__ __forceinline__ u32x4 load_row(const uint16_t* x) {
+  const u32x4* const p = reinterpret_cast<const u32x4*>(x);
+  return MOVE == kAllPast ? __builtin_nontemporal_load(p) : *p;
+}
+template <int MOVE>
+__device__ __forceinline__ void store_row(uint16_t* y, u32x4 v) {
+  if (MOVE == kKept) *reinterpret_cast<u32x4*>(y) = v;
+  else __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(y));
+}
+
 __device__ __forceinline__ float weight_at(const Heads& h, int d) {
   if (h.w == nullptr) return 1.f;
   return h.w16 ? bf16_to_f32(static_cast<const uint16_t*>(h.w)[d]) : static_cast<const float*>(h.w)[d];
@@ -189,7 +207,7 @@ __device__ __forceinline__ void rotate8(const Lane<D, ADJ>& l, u32x4 x, const fl
     y[e] = fmaf(f[e] * r, w[e] * l.c[e], (o[e] * r) * (wo[ADJ ? e ^ 1 : e] * l.s[e]));
 }
 
-template <int D, bool ADJ>
+template <int D, bool ADJ, int MOVE>
 __global__ void __launch_bounds__(256) norm_rotate_kernel(RotateArgs p) {
   using L = Lane<D, ADJ>;
   constexpr int kAhead = 4;
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(RotateArgs p) {
         for (int u = 0; u < kAhead; ++u) {
           const int head = (i + u) * L::kRows + l.sub;
           x[u] = u32x4{0, 0, 0, 0};
-          if (i + u < to && head < h.n) x[u] = ld16(h.x + row * h.xs + head * h.xh + l.d);
+          if (i + u < to && head < h.n) x[u] = load_row<MOVE>(h.x + row * h.xs + head * h.xh + l.d);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -234,7 +252,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(RotateArgs p) {
           float y[8];
           rotate8<D, ADJ>(l, x[u], w, wo, p.eps, y);
           if (head < h.n)
-            *reinterpret_cast<u32x4*>(p.y[t] + ((int64_t)row * h.n + head) * D + l.d) = pack(y);
+            store_row<MOVE>(p.y[t] + ((int64_t)row * h.n + head) * D + l.d, pack(y));
         }
       }
     }
@@ -257,7 +275,7 @@ struct RotateBwdArgs {
   float eps;
 };
 
-template <int D, bool ADJ>
+template <int D, bool ADJ, int MOVE>
 __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(RotateBwdArgs p) {
   using L = Lane<D, ADJ>;
   constexpr int kAhead = 2;
@@ -293,8 +311,8 @@ __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(RotateBwdArgs p) {
           const int head = (i + u) * L::kRows + l.sub;
           x[u] = g[u] = u32x4{0, 0, 0, 0};
           if (i + u < to && head < h.n) {
-            x[u] = ld16(h.x + row * h.xs + head * h.xh + l.d);
-            g[u] = ld16(p.dy[t] + row * p.ds[t] + head * p.dh[t] + l.d);
+            x[u] = load_row<MOVE>(h.x + row * h.xs + head * h.xh + l.d);
+            g[u] = load_row<MOVE>(p.dy[t] + row * p.ds[t] + head * p.dh[t] + l.d);
           }
         }
 #pragma unroll
@@ -326,7 +344,7 @@ __global__ void __launch_bounds__(256) norm_rotate_bwd_kernel(RotateBwdArgs p) {
             for (int e = 0; e < 8; ++e) y[e] = r * fmaf(-f[e], sum, dz[e]);
           }
           if (head < h.n)
-            *reinterpret_cast<u32x4*>(p.dx[t] + ((int64_t)row * h.n + head) * D + l.d) = pack(y);
+            store_row<MOVE>(p.dx[t] + ((int64_t)row * h.n + head) * D + l.d, pack(y));
         }
       }
     }
@@ -472,8 +490,11 @@ __global__ void __launch_bounds__(256) append_rotated_kernel(AppendRotatedArgs p
   }
 }
 
-// Waves that fill the GPU; workgroups of a launch, which take their tokens in turn.
-constexpr int64_t kEnough = 4096, kMostBlocks = 2048, kMostBwdBlocks = 1024;
+// Waves that fill the GPU; workgroups of a launch, which take their tokens in turn: many
+// where each stands alone (a clip of 57,720 tokens, four a workgroup at a time: 543 us
+// with 2,048, 523 with 16,384), few where each leaves sums (24,960 tokens and
+// gradients: 653, 593, 602 with 512, 768, 1,024).
+constexpr int64_t kEnough = 4096, kMostBlocks = 16384, kMostBwdBlocks = 768;
 
 // A launch's parts: waves for `rounds` rounds of every row, all by one where rows
 // are enough to fill the GPU.
@@ -540,6 +561,16 @@ void by_kind(int64_t head_dim, int adjacent, F f) {
   else f(D64{}, std::false_type{});
 }
 
+// And f(head_dim, adjacent, how rows are moved) for `bytes` of them.
+template <typename F>
+void by_kind_and_size(int64_t head_dim, int adjacent, int64_t bytes, F f) {
+  by_kind(head_dim, adjacent, [&](auto d, auto adj) {
+    if (bytes >= (1 << 28)) f(d, adj, std::integral_constant<int, kAllPast>{});
+    else if (bytes >= (1 << 25)) f(d, adj, std::integral_constant<int, kStoresPast>{});
+    else f(d, adj, std::integral_constant<int, kKept>{});
+  });
+}
+
 }  // namespace
 }  // namespace veda
 
@@ -571,8 +602,10 @@ extern "C" int veda_norm_rotate(const void* q, int64_t q_stride_s, int64_t q_str
   p.per_part = split.per_part;
   p.eps = eps;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  by_kind(head_dim, adjacent && n_pairs > 0, [&](auto d, auto adj) {
-    norm_rotate_kernel<decltype(d)::value, decltype(adj)::value><<<split.grid, 256, 0, s>>>(p);
+  const int64_t bytes = 2 * rows * (q_heads + k_heads) * head_dim;
+  by_kind_and_size(head_dim, adjacent && n_pairs > 0, bytes, [&](auto d, auto adj, auto move) {
+    norm_rotate_kernel<decltype(d)::value, decltype(adj)::value, decltype(move)::value>
+        <<<split.grid, 256, 0, s>>>(p);
   });
   return check_launch("veda_norm_rotate");
 }
@@ -622,8 +655,10 @@ extern "C" int veda_norm_rotate_bwd(const void* q, int64_t q_stride_s, int64_t q
   p.eps = eps;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (work) {
-    by_kind(head_dim, adjacent && n_pairs > 0, [&](auto d, auto adj) {
-      norm_rotate_bwd_kernel<decltype(d)::value, decltype(adj)::value><<<split.grid, 256, 0, s>>>(p);
+    const int64_t bytes = 2 * rows * (q_heads + k_heads) * head_dim;
+    by_kind_and_size(head_dim, adjacent && n_pairs > 0, bytes, [&](auto d, auto adj, auto move) {
+      norm_rotate_bwd_kernel<decltype(d)::value, decltype(adj)::value, decltype(move)::value>
+          <<<split.grid, 256, 0, s>>>(p);
     });
     if (int rc = check_launch("veda_norm_rotate_bwd")) return rc;
   }

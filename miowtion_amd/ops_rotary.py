@@ -14,7 +14,7 @@ from miowtion_amd.ops_packed import HEAD_DIMS, _BF16, _F32, _I32, _check_cache, 
 
 _KINDS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 # workgroups of the backward at most, each with sums of its own for the weights
-_BWD_BLOCKS = 1024
+_BWD_BLOCKS = 768
 
 
 def _rotation(rows: int, positions, turns, axes, n_axes: int, interleaved: bool, own: bool, dev: int) -> list:

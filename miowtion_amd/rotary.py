@@ -122,7 +122,9 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     where the formula has them; no other row is touched by it.
     """
     turns, axes, n_axes, interleaved = _parts(rotary)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
+                                    or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         out = _NormRotate.apply(q, k, q_weight, k_weight, positions, turns, axes, n_axes, interleaved, eps)
     else:
         out = ops_rotary.norm_rotate(q, k, positions, turns, axes, n_axes, interleaved, q_weight, k_weight, eps)
