@@ -20,8 +20,9 @@ from miowtion_amd.ops import TILE, _custom_op, _p, _raw_stream
 
 HEAD_DIMS = (64, 128)
 PAGES = (16, 32, 64, 128, 256)
-_CHUNK_WORK = 1 << 27
 _BF16, _F32, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
+# bytes of chunk_fwd's sums at most; sequences up to which its kernel orders them by length
+_CHUNK_WORK, _CHUNK_RANKED = 1 << 27, 126
 # absent from a torch built without a GPU, where no op gets as far as a launch
 _current_device = getattr(torch._C, '_cuda_getDevice', None)
 
@@ -332,16 +333,17 @@ def _(q, k_pages, v_pages, k_exp, v_exp, table, lengths, scale, return_lse):
 
 
 def _chunk_splits(rows: int, heads: int, kv_heads: int, d: int, n_seq: int, capacity: int) -> tuple[int, int]:
-    """(splits of a row's keys at most, workgroups wanted for each key head) of chunk_fwd. How
-    many splits a sequence gets is up to its length, which is on the GPU."""
+    """(splits of a row's keys at most, splits of a key head beyond one of each tile at
+    most) of chunk_fwd. How many a sequence gets is up to the lengths, which are on the GPU;
+    here are the room for it and the grid: splits of 256 keys at least, 128 MB of sums,
+    and no more of them than the lengths can ask for where all are as long as the table
+    (sqrt(W R / (2 s)), with W steps of 64 keys on R places and s = 8)."""
+    room = min(-(-capacity // 256), _CHUNK_WORK // max(4 * rows * heads * (d + 2), 1), 64)
+    if n_seq > _CHUNK_RANKED:  # tiles enough for most; a sequence's splits lie side by side
+        room = min(room, -(-512 // (n_seq * kv_heads)))
     resident = max((512 if d == 128 else 768) // kv_heads, 1)
     tiles = rows * heads // kv_heads // TILE + min(n_seq, rows)
-    units = min(int(math.sqrt(tiles * capacity * resident / 1024)), 2 * resident) + 1
-    if n_seq <= 126:
-        most = min(-(-capacity // 256), _CHUNK_WORK // max(4 * rows * heads * (d + 2), 1), 64)
-    else:
-        most = min(-(-capacity // 256), -(-512 // (n_seq * kv_heads)))
-    return max(most, 1), units
+    return max(room, 1), min(int(math.sqrt(tiles * capacity * resident / 1024)), 2 * resident) + 1
 
 
 @_custom_op('veda::chunk_fwd', mutates_args=())

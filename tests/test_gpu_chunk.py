@@ -125,6 +125,58 @@ def test_long_contexts(d, dtype):
 
 
 @TYPES
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('rows', [15, 16, 17, 31, 32, 33, 127, 128, 129])
+def test_rows_about_the_tiles_sizes(rows, d, dtype):
+    """One head to a key head: as many rows as new tokens, beside a short and a long one."""
+    lens, new = [900, 700, 40], [rows, 1, 40]
+    cache, table, k, v = _filled(lens, 16, 2, d, dtype)
+    q = _queries(sum(new), 2, d)
+    got = kernels.paged_chunk_attention(q, pr.offsets(new), cache, table, _ints(lens), return_lse=True)
+    _check(got, pr.attend(q, k, v, new, lens), dtype)
+
+
+@TYPES
+@pytest.mark.parametrize('heads', [31, 33, 130, 200])
+def test_many_heads_to_a_key_head(heads, dtype):
+    lens, new = [300, 77], [2, 3]
+    cache, table, k, v = _filled(lens, 32, 1, 64, dtype)
+    q = _queries(sum(new), heads, 64)
+    got = kernels.paged_chunk_attention(q, pr.offsets(new), cache, table, _ints(lens), return_lse=True)
+    _check(got, pr.attend(q, k, v, new, lens), dtype)
+
+
+@TYPES
+@pytest.mark.parametrize('n_seq', [126, 127, 140])
+def test_many_sequences_with_long_ones(n_seq, dtype):
+    """About as many sequences as are ordered by length, with keys that are split."""
+    lens = [4000, 1500] + [20] * (n_seq - 3) + [2500]
+    new = [3, 40] + [1] * (n_seq - 3) + [20]
+    cache, table, k, v = _filled(lens, 16, 1, 64, dtype)
+    q = _queries(sum(new), 3, 64)
+    got = kernels.paged_chunk_attention(q, pr.offsets(new), cache, table, _ints(lens), return_lse=True)
+    _check(got, pr.attend(q, k, v, new, lens), dtype)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('new', [[3], [60]])
+@pytest.mark.parametrize('power', [-60, 0, 60])
+def test_e4m3_keys_with_queries_of_every_size(power, new, d):
+    """Values of a query that differ by 2^24 within its blocks of 32, rows of zeros, and rows
+    and keys far from one, whose products are scores as usual."""
+    lens = [400]
+    cache, table, k, v = _filled(lens, 16, 1, d, E4M3, scale=2.0 ** -power)
+    v = v.clone()
+    q = _queries(new[0], 4, d).float()
+    q = q * torch.exp2(-torch.randint(0, 24, q.shape, generator=torch.Generator().manual_seed(2))).cuda()
+    q[..., ::9] = _queries(new[0], 4, d, seed=3).float()[..., ::9]
+    q[0, 1] = 0
+    q = (q * 2.0 ** power).to(BF16)
+    got = kernels.paged_chunk_attention(q, pr.offsets(new), cache, table, _ints(lens), return_lse=True)
+    _check(got, pr.attend(q, k, v, new, lens), E4M3)
+
+
+@TYPES
 def test_unsplit_long_walks(dtype):
     """Enough rows that no key is split, over many windows."""
     lens, new = [9000, 6000], [700, 1030]
