@@ -6,13 +6,20 @@
 // (paged_common.h), in bf16 or e4m3.
 //
 // A wave loads 16 of a step's 64 keys, which lie in one page: pages have 16 rows at
-// least and begin where a block of 16 keys does. A lane holds the page of one step
-// for its wave, 64 steps at a time, so a step's page is one lane's register.
+// least and begin where a block of 16 keys does. A lane holds where the keys of one step
+// lie for its wave, 64 steps at a time, so a step's place is one lane's registers.
 //   bf16: rows go from the page straight into LDS.
-//   e4m3: codes of a step wait in registers for one iteration, while they come, and
-//         are decoded (times the row's power of two: exact) on their way into LDS, once
-//         for the workgroup's 128 rows.
+//   e4m3: codes wait for one iteration, while they come (V's in registers, K's in LDS),
+//         and are decoded (times the row's power of two: exact) on their way into the
+//         slots, once for the workgroup's 128 rows. (Products of the codes themselves, by
+//         the instructions that take e4m3 with a scale for a row and Q as two terms of
+//         it, took 7 to 8 % less time, but cut a product off at 2^-13 of the largest of eight:
+//         an LSE off by 1e-5 where it is off by 1e-7.)
 // A key in a page outside the cache draws no weight.
+//
+// Bound as the packed forward is where rows are many (two chunks of 2,048 onto 32,768 and
+// 20,001, 32 heads on 8, head_dim 128: @A@), by the cache's bytes and a launch's start
+// where they are few (@B@).
 #include <type_traits>
 
 #include "packed_walk.h"
@@ -273,163 +280,7 @@ struct Place {
   uint32_t bad;
 };
 
-// ---------------------------------------------------------------------------
-// e4m3 keys. The products S^T = K Q^T take the cache's codes as they lie, each row
-// with its power of two as the instruction's own scale, and Q as two e4m3 terms:
-// q = (h + l 2^-5) 2^e with one e for 32 dims of a row, h the value rounded to e4m3
-// and l what that leaves. A bf16 value has eight significant bits and either term
-// four, so a value that is at least 2^-13 of the row's largest (of 32) is exact, and
-// what is lost of smaller ones is below 2^-22 of the largest. Two products of e4m3 take
-// the time of one of bf16, K takes half of its room and reads in LDS, and no key is
-// decoded (which would cost as many vector instructions as a third of the softmax).
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-
-// A row's 32 dims from 64 t + 32 (lane / 32) on, for each t.
-template <int D>
-struct Query8 {
-  i32x8 h[D / 64], l[D / 64];
-  uint32_t scale;  // bytes: t 0's h, l, t 1's h, l
-};
-
-// The codes of a lane's 32 dims, four chunks of eight bf16. The instruction's blocks of 32
-// with one scale are the first 16 codes of both lanes of a row, and the last 16: lane
-// 32 h + i gives row i's scale of block h.
-__device__ __forceinline__ void split8(const u32x4 (&x)[4], int half, i32x8& h, i32x8& l, uint32_t& scales) {
-  float up[2];
-  scales = 0;
-#pragma unroll
-  for (int blk = 0; blk < 2; ++blk) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w = x[2 * blk + i / 4][i % 4], lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
-      top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-    }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    // scaled to 128 .. 256 (at an exponent of 12 at least, for l's scale to be one)
-    const uint32_t e = max(top >> 7, 12u);
-    up[blk] = __uint_as_float((261u - e) << 23);
-    if (blk == half) scales = (e - 7) | (e - 12) << 8;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {  // four values at a time
-    float f[4], g[4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const uint32_t w = x[i / 2][2 * (i % 2) + m];
-      f[2 * m] = bf16_to_f32(w & 0xffffu) * up[i / 4];
-      f[2 * m + 1] = bf16_to_f32(w >> 16) * up[i / 4];
-    }
-    int a = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-    a = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], a, true);
-    g[0] = __builtin_amdgcn_cvt_f32_fp8(a, 0);
-    g[1] = __builtin_amdgcn_cvt_f32_fp8(a, 1);
-    g[2] = __builtin_amdgcn_cvt_f32_fp8(a, 2);
-    g[3] = __builtin_amdgcn_cvt_f32_fp8(a, 3);
-    uint32_t odd = 0;  // a NaN or an infinity: a NaN
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const bool ok = fabsf(f[m]) < INFINITY;
-      odd |= ok ? 0u : 0x7fu << (8 * m);
-      g[m] = ok ? (f[m] - g[m]) * 32.f : 0.f;
-    }
-    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(g[0], g[1], 0, false);
-    h[i] = (int)((uint32_t)a | odd);
-    l[i] = __builtin_amdgcn_cvt_pk_fp8_f32(g[2], g[3], c, true);
-  }
-}
-
-// K rows of D codes in LDS, 16-byte chunks permuted by row: chunk c of row r lies at
-// c ^ swz_code<D>(r), so that 16 rows' reads meet every bank once.
-template <int D>
-__device__ __forceinline__ int swz_code(int r) {
-  return D == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
-}
-
-// Addresses of a lane's codes: row li, dims 64 t + 32 hi .. + 31, two chunks each.
-template <int D>
-struct CodeFrags {
-  uint32_t k[D / 32];
-};
-
-__device__ __forceinline__ i32x8 code_frag(const lds_u8* kb, uint32_t a, uint32_t b) {
-  const u32x4 x = *reinterpret_cast<const lds_u32x4*>(kb + a), y = *reinterpret_cast<const lds_u32x4*>(kb + b);
-  return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-}
-
-// s + a term of Q times the codes k; TERM 2 t + (l ? 1 : 0). The result must not share
-// registers with the factors, which hipcc gives it where s is the constant zero and
-// they are used no more: they are used once more.
-template <int D, int TERM>
-__device__ __forceinline__ f32x16 code_product(i32x8 k, uint32_t k_scale, const Query8<D>& q, f32x16 s) {
-  const i32x8 term = (TERM & 1) ? q.l[TERM / 2] : q.h[TERM / 2];
-  const f32x16 r = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, term, s, 0, 0, 0, (int)k_scale, TERM,
-                                                                   (int)q.scale);
-  asm volatile("" : : "v"(k), "v"(term));
-  return r;
-}
-
-// A stage of the walk (packed_walk.h) whose scores are formed so. kb: the sub-block's
-// K rows; ke: its exponents.
-template <int D, bool QK, int SM, bool PV, typename Hook>
-__device__ __forceinline__ void stage8(const lds_u8* kb, const lds_u8* ke, const lds_u8* vb, const Frags<D>& f,
-                                       const CodeFrags<D>& cf, const Query8<D>& q, float c, f32x16& sn,
-                                       const f32x16& sp, u32x4 (&pn)[2], const u32x4 (&pp)[2], Wave<D>& w,
-                                       int li, Hook hook) {
-  using T = Tile<D>;
-  constexpr int kEvery = 8 / T::kK;       // pieces for a product of P V
-  constexpr int kTerms = D / 32;          // products of Q K, one every 8 / kTerms pieces
-  if (PV && __any(w.alpha != 1.f)) {
-#pragma unroll
-    for (int t = 0; t < T::kT; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w.o[t][e] *= w.alpha;
-  }
-  i32x8 kf[D / 64];
-  bf16x8 va[T::kK];
-  uint32_t k_scale = 0;
-  if (QK) {
-    sn = zero16();
-    k_scale = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(ke + 4 * li);
-    kf[0] = code_frag(kb, cf.k[0], cf.k[1]);
-  }
-  if (PV) va[0] = vt_frag<D>(vb, f, 0);
-  float l4[4];
-  const float mu = w.mu;
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    hook(j);
-    const int i = j / kEvery;
-    if (QK && j % (8 / kTerms) == 0) {
-      const int term = j / (8 / kTerms);
-      if (term > 0) asm volatile("" : "+v"(sn));  // formed here, not sunk to its use
-      if (D == 128 && term == 0) kf[D / 64 - 1] = code_frag(kb, cf.k[D / 32 - 2], cf.k[D / 32 - 1]);
-      if (term == 0) sn = code_product<D, 0>(kf[0], k_scale, q, sn);
-      if (term == 1) sn = code_product<D, 1>(kf[0], k_scale, q, sn);
-      if (D == 128 && term == 2) sn = code_product<D, D == 128 ? 2 : 0>(kf[D / 64 - 1], k_scale, q, sn);
-      if (D == 128 && term == 3) sn = code_product<D, D == 128 ? 3 : 0>(kf[D / 64 - 1], k_scale, q, sn);
-    }
-    if (SM != kNoSm) {
-      const float a = __builtin_amdgcn_exp2f(fmaf(sp[2 * j], c, -mu));
-      const float b = __builtin_amdgcn_exp2f(fmaf(sp[2 * j + 1], c, -mu));
-      l4[j >> 1] = (j & 1) ? l4[j >> 1] + (a + b) : a + b;
-      uint32_t pk = pack_bf16x2(a, b);
-      asm volatile("" : "+v"(pk));  // kept here, not sunk to its use a stage later
-      pn[j >> 2][j & 3] = pk;
-    }
-    if (PV && j % kEvery == kEvery - 1) {
-      if (i + 1 < T::kK) va[i + 1] = vt_frag<D>(vb, f, i + 1);
-      w.o[i % T::kT] = mfma32(va[i], as_bf16x8(pp[i / T::kT]), w.o[i % T::kT]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  if (QK) asm volatile("" : "+v"(sn));
-  w.alpha = 1.f;
-  if (SM != kNoSm) take_sums<D, SM>(l4, sp, c, pn, w);
-}
 
 // ---------------------------------------------------------------------------
 // A sequence of at most 32 rows (few new tokens), 16 NB at most: each wave takes tiles of 32 keys of its
@@ -731,13 +582,9 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
 template <int D, bool F8>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkArgs p) {
   using T = Tile<D>;
-  constexpr int kKBytes = F8 ? 64 * D : T::kBytes;  // K of a step
-  constexpr int kSlot = kKBytes + T::kBytes;        // and V, in bf16
-  // (rows of Q pass through slot 1 and what is behind it)
-  constexpr int kRing = F8 ? kSlot + 4 * 32 * T::kPitch : 2 * kSlot;
-  static_assert(kRing >= 2 * kSlot && kRing >= 4 * 32 * T::kPitch, "the ring holds its slots and the rows that leave");
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[kRing];
-  __shared__ uint32_t exps[F8 ? 2 : 1][64];  // of K's rows
+  constexpr int kSlot = 2 * T::kBytes;        // K and V of a step, in bf16
+  constexpr int kRaw = F8 ? 64 * D : 0;       // K's codes of a step
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kSlot + kRaw];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int li = lane & 31, hi = lane >> 5;
@@ -814,76 +661,88 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkA
     return x;
   };
   lds_u8* const s0 = (lds_u8*)ring;
-  lds_u8* const e0 = (lds_u8*)exps;
-  // Rows that go into LDS as they lie: K, and V in bf16. This wave's loads of a step, a
-  // segment is 1 KB of its 16 rows; `clamp`: rows past the sequence's last key read
-  // that key again.
-  constexpr int kKSegs = kKBytes / 4096, kVSegs = T::kSegs;
+  // bf16 rows go into LDS as they lie. This wave's loads of a step's K or V, a segment is
+  // 1 KB of its 16 rows; `clamp`: rows past the sequence's last key read that key again.
+  // e4m3: K's codes, each lane's 16 where it reads them again.
+  constexpr int kSegs = F8 ? D / 64 : T::kSegs;
   struct Src {
     const char* base;
-    uint32_t off[T::kSegs];
+    uint32_t off[kSegs];
   };
   auto src_of = [&](bool is_v, const Place& y, bool clamp) __attribute__((always_inline)) {
     Src r;
     r.base = reinterpret_cast<const char*>(is_v ? vx : kx) + y.at;
-    constexpr int kChunks = F8 ? D / 16 : T::kChunks, kSegRows = 64 / kChunks;
+    constexpr int kChunks = kBytes * D / 16, kSegRows = 64 / kChunks;
 #pragma unroll
-    for (int s = 0; s < (is_v ? kVSegs : kKSegs); ++s) {
+    for (int s = 0; s < kSegs; ++s) {
       const int row = s * kSegRows + lane / kChunks, pos = lane % kChunks;
       const uint32_t src = (uint32_t)(clamp ? min(row, y.rows - 1) : row);
-      const int swz = is_v ? swz_tr<D>(row) : F8 ? swz_code<D>(row) : swz_row<D>(row);
+      const int swz = F8 ? 0 : is_v ? swz_tr<D>(row) : swz_row<D>(row);
       r.off[s] = src * (uint32_t)(kBytes * p.kp.ss) + ((pos ^ swz) << 4);
     }
     return r;
   };
-  const uint32_t lds_k = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(s0 + kKSegs * 1024 * wave));
-  const uint32_t lds_v = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(s0 + kKBytes + kVSegs * 1024 * wave));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(s0 + (F8 ? 2 * kSlot : 0) + kSegs * 1024 * wave));
   auto issue = [&](const Src& x, int s, uint32_t to) { dma16_m0(x.base, x.off[s], to + s * 1024); };
-  // e4m3 values are decoded (times the row's power of two: exact) on their way into LDS,
-  // once for the workgroup's 128 rows: 16 codes of a lane, kCodeLanes lanes a row
+  // e4m3 rows are decoded (times the row's power of two: exact) on their way into the
+  // slots, once for the workgroup's 128 rows: 16 codes of a lane, kCodeLanes lanes a row. V's
+  // codes wait in registers while they come, K's in the wave's part of LDS, as there are
+  // not registers for both.
   constexpr int kCodeLanes = D / 16, kCodes = kCodeLanes / 4;
-  auto exponent = [&](const uint8_t* x, const Place& y, int row, bool clamp) __attribute__((always_inline)) {
-    return exponent_at(x + y.exp + head * p.kp.eh,
-                       (uint32_t)(clamp ? min(row, y.rows - 1) : row) * (uint32_t)p.kp.es);
+  struct Exponents {
+    Exponent of[kCodes > 0 ? kCodes : 1];
   };
   struct Codes {
     u32x4 x[kCodes > 0 ? kCodes : 1];
-    Exponent e[kCodes > 0 ? kCodes : 1];
+    Exponents e;
+  };
+  auto code_row = [&](int s) { return s * (64 / kCodeLanes) + lane / kCodeLanes; };
+  auto exponents = [&](const uint8_t* x, const Place& y, bool clamp) __attribute__((always_inline)) {
+    Exponents r;
+#pragma unroll
+    for (int s = 0; s < kCodes; ++s) {
+      const int row = clamp ? min(code_row(s), y.rows - 1) : code_row(s);
+      r.of[s] = exponent_at(x + y.exp + head * p.kp.eh, (uint32_t)row * (uint32_t)p.kp.es);
+    }
+    return r;
   };
   auto fetch = [&](const Place& y, bool clamp) __attribute__((always_inline)) {
     Codes r;
 #pragma unroll
     for (int s = 0; s < kCodes; ++s) {
-      const int row = s * (64 / kCodeLanes) + lane / kCodeLanes;
-      const uint32_t src = (uint32_t)(clamp ? min(row, y.rows - 1) : row);
+      const uint32_t src = (uint32_t)(clamp ? min(code_row(s), y.rows - 1) : code_row(s));
       r.x[s] = *reinterpret_cast<const u32x4*>(vx + y.at + (src * (uint32_t)p.kp.ss + 16 * (lane % kCodeLanes)));
-      r.e[s] = exponent(p.vp.e, y, row, clamp);
     }
+    r.e = exponents(p.vp.e, y, clamp);
     return r;
   };
-  auto put = [&](const Codes& x, int s, uint32_t slot) __attribute__((always_inline)) {
+  auto put = [&](u32x4 x, const Exponent& e, int s, uint32_t slot, bool is_v) __attribute__((always_inline)) {
     u32x4 a, c;
-    decode16(x.x[s], scale_of(byte_of(x.e[s])), a, c);
-    const int row = 16 * wave + s * (64 / kCodeLanes) + lane / kCodeLanes, ch = 2 * (lane % kCodeLanes);
-    lds_u8* const to = s0 + slot + kKBytes + row * T::kPitch;
-    *reinterpret_cast<lds_u32x4*>(to + ((ch ^ swz_tr<D>(row)) << 4)) = a;
-    *reinterpret_cast<lds_u32x4*>(to + (((ch + 1) ^ swz_tr<D>(row)) << 4)) = c;
+    decode16(x, scale_of(byte_of(e)), a, c);
+    const int row = 16 * wave + code_row(s), ch = 2 * (lane % kCodeLanes);
+    const int swz = is_v ? swz_tr<D>(row) : swz_row<D>(row);
+    lds_u8* const to = s0 + slot + (is_v ? T::kBytes : 0) + row * T::kPitch;
+    *reinterpret_cast<lds_u32x4*>(to + ((ch ^ swz) << 4)) = a;
+    *reinterpret_cast<lds_u32x4*>(to + (((ch + 1) ^ swz) << 4)) = c;
   };
-  auto put_exponents = [&](const Exponent& x, int slot) __attribute__((always_inline)) {
-    if (lane < 16)
-      *reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(e0 + 256 * slot + 64 * wave + 4 * lane) = byte_of(x);
+  auto put_v = [&](const Codes& x, int s, uint32_t slot) __attribute__((always_inline)) {
+    put(x.x[s], x.e.of[s], s, slot, true);
+  };
+  // (K's exponents are asked for behind its codes, and loads arrive in order: once the
+  // former are here so are the latter)
+  auto put_k = [&](Exponents& e, int s, uint32_t slot) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(e.of[s].word) : : "memory");
+    const u32x4 x = *reinterpret_cast<const lds_u32x4*>(s0 + 2 * kSlot + 1024 * (kSegs * wave + s) + 16 * lane);
+    put(x, e.of[s], s, slot, false);
   };
 
   Frags<D> f;
-  CodeFrags<D> cf;
 #pragma unroll
   for (int s = 0; s < T::kK; ++s)
     f.k[s] = (uint32_t)(li * T::kPitch + (((2 * s + hi) ^ swz_row<D>(li)) << 4));
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s)
-    cf.k[s] = (uint32_t)(li * D + (((4 * (s >> 1) + 2 * hi + (s & 1)) ^ swz_code<D>(li)) << 4));
-#pragma unroll
-  for (int t = 0; t < T::kT; ++t) f.v[t] = kKBytes + tr_offset<D>(lane, t, 0, swz_tr<D>);
+  for (int t = 0; t < T::kT; ++t) f.v[t] = T::kBytes + tr_offset<D>(lane, t, 0, swz_tr<D>);
 #pragma unroll
   for (int t = 0; t < T::kT; ++t) w.o[t] = zero16();
   w.m_run = -INFINITY;
@@ -891,169 +750,128 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkA
   w.alpha = 1.f;
   w.have_ref = false;
   const float c = p.scale_log2;
-  Query8<D> q8;
 
   // The walk of the packed forward: iteration u multiplies K of step u + 1 and V of step
-  // u, and brings K of step u + 2 (over K of step u) and V of step u + 1 into LDS, as
-  // loads that have an iteration to arrive; V in e4m3 was asked for an iteration before.
-  constexpr int kSub = 32 * (F8 ? D : T::kPitch), kVSub = 32 * T::kPitch;  // bytes of 32 rows of K, of V
-  Exponent ke;   // e4m3: of K of step u + 1, of row lane % 16
-  auto sync = [&](bool all = true) {
-    if (all) VEDA_WAIT_VM(0);
+  // u, and brings K of step u + 2 (over K of step u) and V of step u + 1 into LDS. bf16:
+  // as loads that have an iteration to arrive. e4m3: as codes that were asked for an
+  // iteration before, which it asks for again, a step on.
+  constexpr int kSub = 32 * T::kPitch;
+  auto sync = [&]() {
     if (F8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the rows that it put into LDS
+    else VEDA_WAIT_VM(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // e4m3: K's exponents of the step are asked for behind its codes, and loads arrive in
-  // order, so once they are here so are the codes; V, asked for behind both, is not
-  // waited for
-  auto sync_codes = [&](uint32_t nxt) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(ke.word));
-    put_exponents(ke, nxt == 0 ? 0 : 1);
-    sync(false);
-  };
   f32x16 sa, sb;
   u32x4 pa[2], pb[2];
-  Place p1;      // of step u + 1
-  Codes vc;      // e4m3: V of step u + 1
-  // both sub-blocks' stages of one step: scores of K at `k`, products with V at `v`
-  auto scores = [&](auto qk, auto sm, auto pv, int sub, uint32_t k, uint32_t v, f32x16& sn, const f32x16& sc,
-                    u32x4 (&pn)[2], const u32x4 (&pp)[2], auto hook) __attribute__((always_inline)) {
-    stage8<D, decltype(qk)::value, decltype(sm)::value, decltype(pv)::value>(
-        s0 + k + sub * kSub, e0 + (k == 0 ? 0 : 256) + 128 * sub, s0 + v + sub * kVSub, f, cf, q8, c, sn, sc, pn, pp, w,
-        li, hook);
-  };
-  using Yes = std::true_type;
-  using No = std::false_type;
-  using NoSm = std::integral_constant<int, kNoSm>;
-  using SmFirst = std::integral_constant<int, kSmFirst>;
-  using SmSecond = std::integral_constant<int, kSmSecond>;
-  auto iter = [&](auto masked, int u, uint32_t cur, uint32_t nxt) __attribute__((always_inline)) {
-    // MASKED: step u + 1 holds keys that some row does not see, or step u + 2 may be past
-    // the last
-    constexpr bool MASKED = decltype(masked)::value;
-    const Place p2 = place(MASKED ? min(u + 2, n_steps - 1) : u + 2);
-    const uint32_t bad = p1.bad;
-    const Src ks = src_of(false, p2, MASKED);
+  Place p1, p2;   // of steps u + 1 and u + 2 (e4m3)
+  Codes vc;       // e4m3: V of step u + 1
+  Exponents ke;   // e4m3: of K of step u + 2
+  constexpr int kAhead = F8 ? 3 : 2;  // the step that K is asked for
+  // Part j of what an iteration brings. e4m3: what is there goes into the slots before
+  // anything is asked for again: V's loads are waited for by their number, and loads into
+  // LDS, which hipcc does not count, would be waited for with them.
+  auto bring = [&](int j, const Src& ks, const Src& vs, const Place& next, bool clamp, uint32_t cur, uint32_t nxt)
+      __attribute__((always_inline)) {
     if constexpr (F8) {
-      sync_codes(nxt);
-      // V of the step first: its loads are waited for by their number, and those that go
-      // into LDS, which hipcc does not count, would be waited for with them
-      auto first = [&](int j) {
-        if (j < kCodes) put(vc, j, nxt);
-        else if (j < kCodes + kKSegs) issue(ks, j - kCodes, lds_k + cur);
-        else if (j == kCodes + kKSegs) ke = exponent(p.kp.e, p2, lane & 15, MASKED);
-        else if (j == kCodes + kKSegs + 1) vc = fetch(p2, MASKED);
-      };
-      scores(Yes{}, SmSecond{}, Yes{}, 0, nxt, cur, sa, sb, pb, pa, first);
-      if (MASKED && 64 * (u + 1) + 32 > wave_all) mask_scores(sa, limit - 64 * (u + 1), hi);
-      if (__builtin_expect((bad & 3) != 0, 0)) mask_blocks(sa, bad);
-      scores(Yes{}, SmFirst{}, Yes{}, 1, nxt, cur, sb, sa, pa, pb, NoHook{});
+      if (j < kCodes) put_k(ke, j, cur);
+      else if (j < 2 * kCodes) put_v(vc, j - kCodes, nxt);
+      else if (j == 2 * kCodes) {
+#pragma unroll
+        for (int s = 0; s < kSegs; ++s) issue(ks, s, lds0);
+        ke = exponents(p.kp.e, next, clamp);
+      } else if (j == 2 * kCodes + 1) {
+        vc = fetch(p2, clamp);
+      }
     } else {
-      const Src vs = src_of(true, p1, MASKED);
-      sync();
-      auto first = [&](int j) {
-        if (j < T::kSegs) issue(ks, j, lds_k + cur);
-        else if (j < 2 * T::kSegs) issue(vs, j - T::kSegs, lds_v + nxt);
-      };
-      Next<D> ahead;
-      stage<D, true, kSmSecond, true, kReadNext>(s0 + nxt, s0 + cur, f, c, sa, sb, pb, pa, w, first, &ahead);
-      if (MASKED && 64 * (u + 1) + 32 > wave_all) mask_scores(sa, limit - 64 * (u + 1), hi);
-      if (__builtin_expect((bad & 3) != 0, 0)) mask_blocks(sa, bad);
-      stage<D, true, kSmFirst, true, kTakeNext>(s0 + nxt + kSub, s0 + cur + kVSub, f, c, sb, sa, pa, pb, w, NoHook{},
-                                                &ahead);
+      if (j < kSegs) issue(ks, j, lds0 + cur);
+      else if (j < 2 * kSegs) issue(vs, j - kSegs, lds0 + nxt + T::kBytes);
     }
+  };
+  auto iter = [&](auto masked, int u, uint32_t cur, uint32_t nxt) __attribute__((always_inline)) {
+    // MASKED: step u + 1 holds keys that some row does not see, or a step that is asked
+    // for may be past the last
+    constexpr bool MASKED = decltype(masked)::value;
+    const Place next = place(MASKED ? min(u + kAhead, n_steps - 1) : u + kAhead);
+    const uint32_t bad = p1.bad;
+    const Src ks = src_of(false, next, MASKED);
+    Src vs;
+    if constexpr (!F8) vs = src_of(true, p1, MASKED);
+    sync();
+    Next<D> ahead;
+    constexpr int kGive = F8 ? kNoNext : kReadNext, kTake = F8 ? kNoNext : kTakeNext;
+    stage<D, true, kSmSecond, true, kGive>(s0 + nxt, s0 + cur, f, c, sa, sb, pb, pa, w,
+                                           [&](int j) { bring(j, ks, vs, next, MASKED, cur, nxt); }, &ahead);
+    if (MASKED && 64 * (u + 1) + 32 > wave_all) mask_scores(sa, limit - 64 * (u + 1), hi);
+    if (__builtin_expect((bad & 3) != 0, 0)) mask_blocks(sa, bad);
+    stage<D, true, kSmFirst, true, kTake>(s0 + nxt + kSub, s0 + cur + kSub, f, c, sb, sa, pa, pb, w, NoHook{},
+                                          &ahead);
     if (MASKED && 64 * (u + 1) + 64 > wave_all) mask_scores(sb, limit - 64 * (u + 1) - 32, hi);
     if (__builtin_expect((bad & 12) != 0, 0)) mask_blocks(sb, bad >> 2);
-    p1 = p2;
+    p1 = F8 ? p2 : next;
+    p2 = next;
   };
-  // A wave without rows (in the tile of a few tokens) only brings keys and values.
-  const bool idle = r0 + 32 * wave >= rows;
-  auto bring = [&](int u, uint32_t cur, uint32_t nxt) __attribute__((always_inline)) {
-    const Place p2 = place(min(u + 2, n_steps - 1));
-    if constexpr (F8) sync_codes(nxt);
-    else sync();
-    const Src ks = src_of(false, p2, true);
-    if constexpr (F8) {
-#pragma unroll
-      for (int s = 0; s < kCodes; ++s) put(vc, s, nxt);
-    }
-#pragma unroll
-    for (int s = 0; s < kKSegs; ++s) issue(ks, s, lds_k + cur);
-    if constexpr (F8) {
-      ke = exponent(p.kp.e, p2, lane & 15, true);
-      vc = fetch(p2, true);
-    } else {
-      const Src vs = src_of(true, p1, true);
-#pragma unroll
-      for (int s = 0; s < kVSegs; ++s) issue(vs, s, lds_v + nxt);
-    }
-    p1 = p2;
-  };
+  const bool idle = r0 + 32 * wave >= rows;  // without rows, in a sequence's last tile: only brings keys and values
   if (n_steps > 0) {
     const Place p0 = place(0);
     p1 = place(min(1, n_steps - 1));
-    {
-      const Src k0 = src_of(false, p0, true);
+    p2 = place(min(2, n_steps - 1));
+    const Src k0 = src_of(false, p0, true);
 #pragma unroll
-      for (int s = 0; s < kKSegs; ++s) issue(k0, s, lds_k);
-    }
+    for (int s = 0; s < kSegs; ++s) issue(k0, s, lds0);
     if constexpr (F8) {
-      const Exponent k_exp = exponent(p.kp.e, p0, lane & 15, true);
+      ke = exponents(p.kp.e, p0, true);
       vc = fetch(p0, true);
 #pragma unroll
-      for (int s = 0; s < kCodes; ++s) put(vc, s, 0);
-      put_exponents(k_exp, 0);
+      for (int s = 0; s < kCodes; ++s) {
+        put_k(ke, s, 0);
+        put_v(vc, s, 0);
+      }
+      const Src k1 = src_of(false, p1, true);
+#pragma unroll
+      for (int s = 0; s < kSegs; ++s) issue(k1, s, lds0);
+      ke = exponents(p.kp.e, p1, true);
+      vc = fetch(p1, true);
     } else {
       const Src v0 = src_of(true, p0, true);
 #pragma unroll
-      for (int s = 0; s < kVSegs; ++s) issue(v0, s, lds_v);
+      for (int s = 0; s < kSegs; ++s) issue(v0, s, lds0 + T::kBytes);
     }
     // Q by way of slot 1, which K of step 1 comes into after the barrier
-    lds_u8* const box = s0 + kSlot + wave * 32 * T::kPitch;
-    frags_of_rows<D>(qrows, box, lane, w.qf);
-    if constexpr (F8) {
-      q8.scale = 0;
+    frags_of_rows<D>(qrows, s0 + kSlot + wave * 32 * T::kPitch, lane, w.qf);
 #pragma unroll
-      for (int t = 0; t < D / 64; ++t) {
-        u32x4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = *reinterpret_cast<const lds_u32x4*>(box + li * T::kPitch + (((8 * t + 4 * hi + i) ^ swz_row<D>(li)) << 4));
-        uint32_t scales;
-        split8(x, hi, q8.h[t], q8.l[t], scales);
-        q8.scale |= scales << (16 * t);
-      }
-      asm volatile("" ::: "memory");
-    } else {
-#pragma unroll
-      for (int s = 0; s < T::kK; ++s) asm volatile("" : : "v"(w.qf[s]));
-    }
+    for (int s = 0; s < T::kK; ++s) asm volatile("" : : "v"(w.qf[s]));
     sync();
-    if (n_steps > 1) {
+    if constexpr (F8) {
+#pragma unroll
+      for (int s = 0; s < kCodes; ++s) put_k(ke, s, kSlot);
+      const Src k2 = src_of(false, p2, true);
+#pragma unroll
+      for (int s = 0; s < kSegs; ++s) issue(k2, s, lds0);
+      ke = exponents(p.kp.e, p2, true);
+    } else if (n_steps > 1) {
       const Src k1 = src_of(false, p1, true);
 #pragma unroll
-      for (int s = 0; s < kKSegs; ++s) issue(k1, s, lds_k + kSlot);
-      if constexpr (F8) {  // behind K's codes: see sync_codes
-        ke = exponent(p.kp.e, p1, lane & 15, true);
-        vc = fetch(p1, true);
-      }
+      for (int s = 0; s < kSegs; ++s) issue(k1, s, lds0 + kSlot);
     }
     if (idle) {
 #pragma unroll 1
       for (int u = 0; u + 1 < n_steps; ++u) {
-        const uint32_t to = (u & 1) * kSlot;
-        bring(u, to, kSlot - to);
+        const uint32_t cur = (u & 1) * kSlot, nxt = kSlot - cur;
+        const Place next = place(min(u + kAhead, n_steps - 1));
+        const Src ks = src_of(false, next, true);
+        Src vs;
+        if constexpr (!F8) vs = src_of(true, p1, true);
+        sync();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bring(j, ks, vs, next, true, cur, nxt);
+        p1 = F8 ? p2 : next;
+        p2 = next;
       }
       sync();
     } else {
-      if constexpr (F8) {
-        scores(Yes{}, NoSm{}, No{}, 0, 0, 0, sa, sb, pa, pb, NoHook{});
-        scores(Yes{}, NoSm{}, No{}, 1, 0, 0, sb, sa, pa, pb, NoHook{});
-      } else {
-        stage<D, true, kNoSm, false>(s0, s0, f, c, sa, sb, pa, pb, w, NoHook{});
-        stage<D, true, kNoSm, false>(s0 + kSub, s0, f, c, sb, sa, pa, pb, w, NoHook{});
-      }
+      stage<D, true, kNoSm, false>(s0, s0, f, c, sa, sb, pa, pb, w, NoHook{});
+      stage<D, true, kNoSm, false>(s0 + kSub, s0, f, c, sb, sa, pa, pb, w, NoHook{});
       if (n_plain == 0) {
         mask_scores(sa, limit, hi);
         mask_scores(sb, limit - 32, hi);
@@ -1065,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkA
       first_reference<D>(sa, sb, c, w);
       stage<D, false, kSmFirst, false>(s0, s0, f, c, sb, sa, pa, pb, w, NoHook{});
       int u = 0;
-      for (; u + 3 < n_plain; u += 2) {
+      for (; u + kAhead + 1 < n_plain; u += 2) {
         iter(std::false_type{}, u, 0, kSlot);
         iter(std::false_type{}, u + 1, kSlot, 0);
       }
@@ -1077,8 +895,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2) chunk_kernel(ChunkA
       const lds_u8* const cur = s0 + ((n_steps - 1) & 1) * kSlot;
       sync();
       stage<D, false, kSmSecond, true>(s0, cur, f, c, sb, sb, pb, pa, w, NoHook{});
-      stage<D, false, kNoSm, true>(s0, cur + kVSub, f, c, sa, sb, pa, pb, w, NoHook{});
+      stage<D, false, kNoSm, true>(s0, cur + kSub, f, c, sa, sb, pa, pb, w, NoHook{});
     }
+    if (F8) VEDA_WAIT_VM(0);  // codes that no step takes are on their way into LDS, which is another's after the end
   }
   if (p.n_split > 1 && unit.split == 0 && real && hi == 0) {
     const int64_t n_heads = (int64_t)p.pk.n_kv * p.pk.group, all_rows = p.pk.q_rows * n_heads;

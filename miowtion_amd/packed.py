@@ -216,10 +216,7 @@ def paged_chunk_attention(q: torch.Tensor, cu: torch.Tensor, cache: PagedCache, 
         out [T, H, D] bf16, or (out, lse). Rows that see no key, and rows of no sequence,
         have out 0 and lse -inf. A key that a row does not see does not touch its out,
         whatever it holds. The same bits on every call with these shapes and lengths.
-        Rounded as packed_attention's. Scores with keys in e4m3 are off by 2^-16 of the sum
-        of their products' magnitudes by square mean (2^-10 at most), for the matrix
-        instructions cut products off at 2^-13 of the largest of eight: less than a
-        hundredth of what the probabilities' rounding to bf16 is.
+        Rounded as packed_attention's.
 
     Rows that meet a NaN or an infinity in v that the mask hides within their tile are
     formed key by key, as packed_attention's. Without gradients, as the cache has none.
