@@ -509,9 +509,10 @@ struct Split {
 };
 Split split_of(int64_t rows, int rounds, int64_t enough, int64_t most) {
   int64_t parts = enough / (rows > 0 ? rows : 1);
-  parts = parts < 1 ? 1 : parts > rounds ? rounds : parts;
+  if (parts > rounds) parts = rounds;
+  if (parts < 1) parts = 1;  // (no heads: no rounds)
   const int per = (int)((rounds + parts - 1) / parts);
-  parts = (rounds + per - 1) / per;
+  if (per > 0) parts = (rounds + per - 1) / per;
   const int64_t blocks = (rows * parts + 3) / 4;
   return Split{(int32_t)parts, per, (unsigned)(blocks < most ? blocks : most)};
 }

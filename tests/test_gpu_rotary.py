@@ -163,6 +163,17 @@ def test_gradients_of_some_inputs():
     rr.within(gx, want['dx'], want['dx_tol'])
 
 
+@pytest.mark.parametrize('rows,heads,kv', [(0, 5, 2), (9, 0, 0), (9, 5, 0), (9, 0, 2), (0, 0, 0)])
+def test_gradients_of_nothing(rows, heads, kv):
+    """No rows, no heads: weights' gradients are zeros where no row is."""
+    q, k, _, wq, wk = _inputs(rows, heads, kv, 128)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, wq, wk)]
+    out = kernels.norm_rotate(*leaves[:2], _positions(rows, 1, torch.int32), kernels.rotary(64), *leaves[2:], 1e-6)
+    got = torch.autograd.grad(out, leaves, [torch.ones_like(t) for t in out])
+    for x, n, g, w in zip(leaves, (heads, kv), got, got[2:]):
+        assert g.shape == x.shape and bool(w.any()) == (rows * n > 0)
+
+
 def test_gradients_that_are_views():
     """Output gradients in strides of their own, expanded ones among them."""
     q, k, _, wq, wk = _inputs(65, 4, 2, 64)

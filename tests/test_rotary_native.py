@@ -88,6 +88,12 @@ def test_calls_without_work_launch_nothing():
     _chunk(rows=0)
 
 
+@pytest.mark.parametrize('rows', [0, 1, 5000])
+def test_gradients_of_no_heads_launch_nothing(rows):
+    _native.call('veda_norm_rotate_bwd', X, 1024, 128, X, 1024, 128, 0, None, 0, 0, None, 0, 0, 0, rows, 128, *_turn(), X,
+                 None, None, None, None, 0, None)
+
+
 def _cpu(*shape, dtype=BF16):
     return torch.zeros(*shape, dtype=dtype)
 
