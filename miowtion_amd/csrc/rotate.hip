@@ -94,6 +94,7 @@ struct Lane {
   int partner;  // the lane of the other dims of the pairs
   int other;    // their first dim (adjacent pairs: d)
   int pair;     // the first pair
+  uint32_t paired;  // all ones where its dims have pairs; adjacent: bit e where dim e has one
   float c[8], s[8];
 
   __device__ __forceinline__ Lane(int l, int pairs) : lane(l), sub(l / kLanes), d(8 * (l % kLanes)) {
@@ -102,6 +103,7 @@ struct Lane {
     partner = lane + step / 8;
     other = d + step;
     pair = ADJ ? d / 2 : region == 2 ? 0 : d - region * pairs;
+    paired = ADJ ? (1u << min(max(2 * pairs - d, 0), 8)) - 1u : region == 2 ? 0u : ~0u;
   }
 
   // Angles from the wave's box; s has the sign that the partner's value takes.
@@ -114,13 +116,21 @@ struct Lane {
     }
   }
 
-  // The other dims of the pairs of a row of packed bf16.
+  // The other dims of the pairs of a row of packed bf16; zero for a dim of no pair, whose
+  // infinities and NaN are its own. Their weights too.
   __device__ __forceinline__ u32x4 partners(u32x4 x) const {
     u32x4 y;
 #pragma unroll
     for (int m = 0; m < 4; ++m)
-      y[m] = ADJ ? (x[m] >> 16) | (x[m] << 16) : (uint32_t)__shfl((int)x[m], partner);
+      y[m] = (ADJ ? (x[m] >> 16) | (x[m] << 16) : (uint32_t)__shfl((int)x[m], partner)) & mask(2 * m);
     return y;
+  }
+  __device__ __forceinline__ float other_weight(const float* weights, int e) const {
+    return __uint_as_float(__float_as_uint(weights[other + e]) & mask(e));
+  }
+  // All ones where dim e has a pair.
+  __device__ __forceinline__ uint32_t mask(int e) const {
+    return ADJ ? (uint32_t)__builtin_amdgcn_sbfe((int)paired, e, 1) : paired;
   }
 };
 
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(RotateArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         w[e] = weights[t][l.d + e];
-        wo[e] = weights[t][l.other + e];
+        wo[e] = l.other_weight(weights[t], e);
       }
       for (int i = from; i < to; i += kAhead) {
         u32x4 x[kAhead];
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(256) append_rotated_kernel(AppendRotatedArgs p
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         w[e] = weights[t & 1][l.d + e];
-        wo[e] = weights[t & 1][l.other + e];
+        wo[e] = l.other_weight(weights[t & 1], e);
       }
       for (int i = from; i < to; i += kAhead) {
         u32x4 x[kAhead];

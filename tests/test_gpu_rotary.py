@@ -114,6 +114,28 @@ def test_large_small_and_not_finite_rows():
     rr.within(torch.where(bad, 0.0, got.double()), torch.where(bad, 0.0, want), torch.where(bad, 1.0, tol))
 
 
+@pytest.mark.parametrize('d,pairs,interleaved', [(128, 8, False), (128, 7, True), (64, 0, False), (64, 13, True)])
+def test_dims_of_no_pair_are_apart(d, pairs, interleaved):
+    """An infinity or a NaN in a dim of no pair, its weight or its gradient: in no other dim."""
+    rot = kernels.rotary(pairs, interleaved=interleaved) if pairs else None
+    q, _, _, wq, _ = _inputs(12, 3, 1, d)
+    pos = _positions(12, 1, torch.int32) if pairs else None
+    x, w = q.clone(), wq.clone()
+    for i in range(12):
+        x[i, i % 3, d - 1 - i] = (math.inf, -math.inf, math.nan)[i % 3]
+    w[d - 3], w[d - 8] = math.inf, math.nan
+    for a, b, eps in ((x, None, None), (x, wq, 1e-6), (q, w, 1e-6)):
+        got, (want, tol) = kernels.norm_rotate(a, None, pos, rot, b, eps=eps)[0].double(), rr.norm_rotate(a, pos, rot, b, eps)
+        odd = ~torch.isfinite(want)
+        assert odd.any() and torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got[odd].nan_to_num(7.0), want[odd].nan_to_num(7.0))
+        rr.within(torch.where(odd, 0.0, got), torch.where(odd, 0.0, want), torch.where(odd, 1.0, tol))
+    leaf = q.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(kernels.norm_rotate(leaf, None, pos, rot)[0], leaf, x)
+    want = rr.gradients(q, pos, rot, None, None, x)['dx']
+    assert torch.equal(torch.isnan(dx), torch.isnan(want)) and torch.equal(torch.isinf(dx), torch.isinf(want))
+
+
 @pytest.mark.parametrize('d,sections,interleaved', [(128, [64], False), (128, [16, 24, 24], True), (64, [8, 8], False),
                                                     (64, [32], True), (128, None, False)])
 @pytest.mark.parametrize('rows,heads,kv', [(1, 1, 1), (77, 5, 2), (611, 8, 2), (5000, 6, 6)])
