@@ -49,8 +49,8 @@ def _device_arch(device: torch.device) -> str:
 def supports(x: torch.Tensor, op: str = 'gather') -> bool:
     """Whether the kernels of `op` ('gather' for gather / pool / scatter,
     'attention' for the sparse and dense forwards, their backward and the
-    compensation, 'heat' for the block heat, 'packed' for packed sequences and
-    the paged cache) can take this tensor: the
+    compensation, 'heat' for the block heat, 'packed' for packed sequences, the
+    paged cache and norms with rotation) can take this tensor: the
     library loads, x is a bf16 tensor with a unit last stride and a head_dim
     that family implements, on a gfx950 device. The routing predicate of
     tile_gather_triton.py:55-66: a caller with another path falls through to
