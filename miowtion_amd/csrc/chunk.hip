@@ -21,9 +21,14 @@
 // 32,768 and 20,001, 32 heads on 8, head_dim 128: 1,460 to 1,520 us, 1.14 PFLOP/s; 1,640 in
 // e4m3, which takes a tenth more LDS accesses and a fifth more vector instructions);
 // where they are few, by the cache's bytes (four tokens of eight sequences over 40,103
-// positions in all, 8 key heads: 34 us, 4.8 TB/s); between them in e4m3 by latency, as half as
-// many bytes are on their way as in bf16 (9 tokens of 64 sequences of 4,096: 152 us, 3.6
-// TB/s, 2.3 us an iteration; in bf16 220 us, 4.9 TB/s).
+// positions in all, 8 key heads: 34 us, 4.8 TB/s); between them in e4m3 by latency, of an
+// iteration's chain and of its loads (9 tokens of 64 sequences of 4,096: 152 us, 3.6 TB/s, 2.3
+// us an iteration, of half of bf16's bytes, which takes 220 us, 4.9 TB/s; with codes asked for
+// two steps ahead, but no products among the softmax, as LDS has not room for both: 179 us).
+// A workgroup takes one unit. Equal shares of all tiles' steps for as many workgroups as
+// are resident, tiles cut where a share ends, took longer (40 on 8 heads, 16 tokens of 48
+// sequences: 62 us for 53; four chunks of 512, head_dim 64: 162 for 131): starts and ends
+// cost 6 to 11 us each, and the tiles of a sequence read their keys at different times.
 #include <type_traits>
 
 #include "packed_walk.h"
