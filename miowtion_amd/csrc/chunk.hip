@@ -530,10 +530,8 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& p, const Unit& unit, c
     for (int w = 0; w < 4; ++w) m = fmaxf(m, red_m[w][r]);
     const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(red_m[w][r] - mu);
-      l = f == 0.f ? l : fmaf(red_l[w][r], f, l);
-    }
+    for (int w = 0; w < 4; ++w)  // (a wave whose scores are all NaN has no reference, but a sum that is NaN)
+      l = fmaf(red_l[w][r], __builtin_amdgcn_exp2f(red_m[w][r] - mu), l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int rr = min(r, rows - 1);
     const int64_t tok = of.query(rr), hd = of.head(rr);

@@ -407,3 +407,82 @@ def test_refusals():
     refused('scale', 4, n, scale=0.0)
     with pytest.raises(NotImplementedError):
         kernels.paged_chunk_attention(*[t.cpu() if isinstance(t, torch.Tensor) else t for t in ok])
+
+
+def _put_nan(cache, table, b, pos, head, dim):
+    """A NaN in dim `dim` of the key of position `pos` of sequence b."""
+    page = cache.k.shape[1]
+    x = cache.k[int(table[b, pos // page]), pos % page, head]
+    if x.dtype == E4M3:
+        x.view(torch.uint8)[dim] = 0x7f
+    else:
+        x[dim] = math.nan
+
+
+def _check_around(got, clean, nan):
+    """NaN in out and LSE of the rows of `nan` [rows, heads], nothing else changed by it."""
+    out, lse = got
+    assert torch.equal(torch.isnan(lse), nan), f'{int((torch.isnan(lse) != nan).sum())} LSEs'
+    assert torch.equal(torch.isnan(out), nan[..., None].expand_as(out)), f'{int((torch.isnan(out).all(-1) != nan).sum())} rows'
+    rr.within(torch.where(nan[..., None], 0.0, out.double()), torch.where(nan[..., None], 0.0, clean['out']),
+              clean['out_tol'])
+    none = clean['lse'] == -math.inf
+    assert (lse[none] == -math.inf).all()
+    rr.within(torch.where(nan | none, 0.0, lse.double()), torch.where(nan | none, 0.0, clean['lse']), clean['lse_tol'])
+
+
+# two query heads to a key head: up to 16 rows, up to 32 and more, keys whole and in splits
+NAN_ROWS = pytest.mark.parametrize('new', [1, 5, 12, 40])
+NAN_LENS = [(1, 0), (33, 32), (65, 64), (97, 96), (129, 40), (5000, 4999), (5000, 300)]
+
+
+@TYPES
+@NAN_ROWS
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('length,bad', NAN_LENS, ids=[f'{b}of{n}' for n, b in NAN_LENS])
+def test_a_key_that_is_nan(length, bad, d, new, dtype):
+    """Every row that sees it is NaN, whichever keys of the row's tiles are beside it, and no
+    other row; also where the keys beside it weigh nothing."""
+    lens, news = [length, 200], [new, 3]
+    cache, table, k, v = _filled(lens, 16, 2, d, dtype)
+    q = _queries(sum(news), 4, d)
+    _put_nan(cache, table, 0, bad, 1, 5)
+    got = kernels.paged_chunk_attention(q, pr.offsets(news), cache, table, _ints(lens), return_lse=True)
+    sees = torch.arange(new) + length - new >= bad
+    nan = torch.zeros(sum(news), 4, dtype=torch.bool)
+    nan[:new, 2:] = sees[:, None]
+    _check_around(got, pr.attend(q, k, v, news, lens), nan.cuda())
+
+
+@TYPES
+@NAN_ROWS
+def test_a_nan_beside_keys_that_weigh_nothing(new, dtype):
+    """The other keys of its 32 have scores some 180 below the rest: probabilities of zero in
+    32 bits."""
+    lens = [400]
+    cache, table, k, v = _filled(lens, 16, 1, 128, dtype)
+    q = torch.full((new, 2, 128), 4.0, dtype=BF16, device='cuda')
+    low = torch.full((32, 1, 128), -4.0, dtype=BF16, device='cuda')  # scores of -181
+    kernels.cache_append_(cache, low, v[64:96].contiguous(), pr.offsets([32]), table, _ints([64]))
+    k = k.clone()
+    k[64:96] = low
+    _put_nan(cache, table, 0, 70, 0, 9)
+    got = kernels.paged_chunk_attention(q, pr.offsets([new]), cache, table, _ints(lens), return_lse=True)
+    _check_around(got, pr.attend(q, k, v, [new], lens), torch.ones(new, 2, dtype=torch.bool, device='cuda'))
+
+
+@TYPES
+@NAN_ROWS
+@pytest.mark.parametrize('length', [1, 33, 200, 5000])
+def test_a_query_that_is_nan(length, new, dtype):
+    """The row is NaN where it sees a key; a row that sees none is as ever."""
+    lens, news = [length, 200], [new, 3]
+    cache, table, k, v = _filled(lens, 16, 2, 128, dtype)
+    q = _queries(sum(news), 4, 128)
+    clean = pr.attend(q, k, v, news, lens)
+    nan = torch.zeros(sum(news), 4, dtype=torch.bool, device='cuda')
+    for row, head in ((0, 1), (new - 1, 1), (new // 2, 3), (new, 0)):
+        q[row, head, 7] = math.nan
+        nan[row, head] = clean['lse'][row, head] != -math.inf
+    got = kernels.paged_chunk_attention(q, pr.offsets(news), cache, table, _ints(lens), return_lse=True)
+    _check_around(got, clean, nan)
