@@ -486,3 +486,24 @@ def test_a_query_that_is_nan(length, new, dtype):
         nan[row, head] = clean['lse'][row, head] != -math.inf
     got = kernels.paged_chunk_attention(q, pr.offsets(news), cache, table, _ints(lens), return_lse=True)
     _check_around(got, clean, nan)
+
+
+@TYPES
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('new', [5, 40])
+def test_lengths_past_the_table_are_its_width(new, causal, dtype):
+    """All of 7 pages' 112 positions are finite, and so are those of the pages that lie
+    behind them in the table's memory; two more pages are outside the cache."""
+    cache, table, k, v = _filled([112, 112], 16, 2, 64, dtype)
+    q = _queries(new, 4, 64)
+    behind = torch.cat([table[:1], table[1:]], 1)  # 14 pages, of which 7 are given
+    outside = torch.cat([table[:1], torch.full((1, 2), -1, dtype=torch.int32, device='cuda')], 1)
+    for n in (113, 144, 1 << 30, (1 << 31) - 1):
+        got = kernels.paged_chunk_attention(q, pr.offsets([new]), cache, behind[:, :7], _ints([n]), causal,
+                                            return_lse=True)
+        _check(got, pr.attend(q, k[:112], v[:112], [new], [112], causal))
+        # the last query is at position min(n, 144) - 1, the keys end at 112
+        got = kernels.paged_chunk_attention(q, pr.offsets([new]), cache, outside, _ints([n]), causal,
+                                            return_lse=True)
+        seen = [min(min(n, 144) - new + i + 1, 112) if causal else 112 for i in range(new)]
+        _check(got, pr.attend(q, *(torch.cat([t[:m] for m in seen]) for t in (k, v)), [1] * new, seen))
