@@ -317,6 +317,54 @@ def test_append_in_eight_bits(d, kv, normed):
         i0, j0 = i0 + m, j0 + n
 
 
+def _codes(x, e):
+    """x [.., D] in 64 bits as e4m3 values at the exponents e [..], rounded once."""
+    y = x / torch.exp2(e - 127)[..., None]
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(y / step) * step
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('normed', [True, False])
+def test_append_in_eight_bits_rounds_once(d, normed):
+    """Codes and exponents of the keys are those of the value in 64 bits, wherever what 32
+    bits may be off by leaves no other; by way of bf16 they are not."""
+    lens, new, kv = [300, 130], [300, 117], 4
+    q, k, v, wq, wk = _inputs(sum(new), kv, kv, d)
+    if not normed:
+        wq = wk = None
+    eps = 1e-6 if normed else None
+    rot = kernels.rotary(d // 2)
+    cache, table = _cache(lens, 32, kv, d, E4M3)
+    other = kernels.PagedCache(*(t.clone() for t in cache))
+    start, cu = _starts(lens, new), pr.offsets(new)
+    kernels.cache_append_rotated_(cache, q, k, v, cu, table, start, rot, None, wq, wk, eps)
+    at = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, new)]).cuda()
+    kernels.cache_append_(other, kernels.norm_rotate(q, k, at, rot, wq, wk, eps)[1], v, cu, table, start)
+
+    want, tol = rr.norm_rotate(k, at, rot, wk, eps)
+    tol = tol - rr.H * want.abs()  # what 32 bits are off by
+    top, off = want.abs().amax(-1), tol.amax(-1)
+    lo, e, up = (127 + torch.ceil(torch.log2(t / 448)) for t in (top - off, top, top + off))
+    sure_row = (lo == e) & (e == up)
+    codes = _codes(want, e)
+    sure = sure_row[..., None] & (_codes(want - tol, e) == codes) & (_codes(want + tol, e) == codes)
+    # a row is at a power's border in one of 2^13 cases, a value of a code's step, 2^-4 to
+    # 2^-3 of it, in one of 2^11 where it is as large as its pair's other
+    assert sure_row.float().mean() > 0.99 and sure.float().mean() > 0.98
+    seq = torch.cat([torch.full((m,), b) for b, m in enumerate(new)]).cuda()
+    page = table[seq, at // 32].long()
+
+    def found(c):
+        return c.k[page, at % 32].double(), c.k_exp[page, at % 32]
+
+    held, power = found(cache)
+    assert torch.equal(power[sure_row].double(), e[sure_row])
+    assert torch.equal(held[sure], codes[sure])
+    held, power = found(other)
+    assert (held[sure] != codes[sure]).any()
+
+
 @pytest.mark.parametrize('dtype', [BF16, E4M3])
 def test_append_leaves_out_what_has_no_page(dtype):
     lens = [20, 20, 20]
