@@ -5,7 +5,7 @@ on streams at once; and rows enough to be moved past the caches."""
 import pytest
 import torch
 
-from miowtion_amd import kernels, ops_rotary
+from miowtion_amd import kernels, ops_packed, ops_rotary
 from tests import packed_reference as pr
 from tests import rotary_reference as rr
 
@@ -144,3 +144,93 @@ def test_rows_that_are_moved_past_the_caches(rows, interleaved):
         # of two pairs' |dy| |x r|, below 4 by square mean each: both sides' sums in 32 bits
         most = 2 * dy.float().abs().mean() * 1.2 * x.shape[0] * x.shape[1]
         assert (s - t.double()).abs().max() <= 2 * (rr.S + rr.LONG) * most
+
+
+def test_different_calls_on_two_streams_at_once():
+    """Every operator of the path, each stream with values and lengths of its own in the same
+    shapes, keys in several splits and weights with gradients: what one call keeps in
+    buffers is no other's."""
+    heads, kv, d, new = 8, 2, 128, [40, 3]
+    rot = kernels.rotary(64)
+    cases = []
+    for seed, lens in ((1, [1500, 2000]), (2, [900, 700])):
+        g = torch.Generator().manual_seed(seed)
+        q, k, v, dq, dk = (torch.randn(sum(new), h, d, generator=g).to(BF16).cuda() for h in (heads, kv, kv, heads, kv))
+        wq, wk = ((1 + 0.2 * torch.randn(d, generator=g)).cuda() for _ in range(2))
+        cache = kernels.paged_cache(256, 16, kv, d)
+        for t in cache[:2]:
+            t.copy_(torch.randn(t.shape, generator=g))
+        table = torch.randperm(256, generator=g).to(torch.int32).view(2, 128).cuda()
+        lengths = torch.tensor(lens, dtype=torch.int32, device='cuda')
+        start = lengths - torch.tensor(new, dtype=torch.int32, device='cuda')
+        pos = torch.randint(0, 9999, (sum(new),), generator=g).cuda()
+        cases.append((q, k, v, dq, dk, wq, wk, cache, table, start, lengths, pos))
+    assert ops_packed._chunk_splits(sum(new), heads, kv, d, 2, 128 * 16)[0] > 1
+    cu = pr.offsets(new)
+
+    def step(case):
+        q, k, v, dq, dk, wq, wk, cache, table, start, lengths, pos = case
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
+        out = kernels.norm_rotate(*leaves[:2], pos, rot, *leaves[2:], 1e-6)
+        grads = torch.autograd.grad(out, leaves, (dq, dk))
+        y = kernels.cache_append_rotated_(cache, q, k, v, cu, table, start, rot, None, wq, wk, 1e-6)
+        return (*[t.detach() for t in out], *grads, y,
+                *kernels.paged_chunk_attention(y, cu, cache, table, lengths, return_lse=True))
+
+    want = [step(case) for case in cases]
+    assert not any(torch.equal(a, b) for a, b in zip(*want))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for mine, case, stream in zip(got, cases, streams):
+            with torch.cuda.stream(stream):
+                mine.append(step(case))
+    torch.cuda.synchronize()
+    for mine, w in zip(got, want):
+        for found in mine:
+            assert all(torch.equal(a, b) for a, b in zip(found, w))
+
+
+@pytest.mark.parametrize('dtype', [BF16, E4M3], ids=['bf16', 'e4m3'])
+def test_compiled(dtype):
+    """The public functions within torch.compile: the same bits, the ops in its graph."""
+    q, k, v, wq, wk, cache, table, start, lengths, pos, rot, cu = _case(dtype)
+    seen = []
+
+    def backend(graph, _):
+        seen.extend(str(n.target) for n in graph.graph.nodes)
+        return graph.forward
+
+    def serve(q, k, v, lengths):
+        y, z = kernels.norm_rotate(q, k, pos, rot, wq, wk, 1e-6)
+        x = kernels.cache_append_rotated_(cache, q, k, v, cu, table, start, rot, pos, wq, wk, 1e-6)
+        return y, z, x, *kernels.paged_chunk_attention(x, cu, cache, table, lengths, return_lse=True)
+
+    want = serve(q, k, v, lengths)
+    held = [None if t is None else t.view(torch.uint8).clone() for t in cache]
+    for t in cache:
+        if t is not None:
+            t.view(torch.uint8).zero_()
+    got = torch.compile(serve, backend=backend, fullgraph=True)(q, k, v, lengths)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(a is None or torch.equal(a.view(torch.uint8), b) for a, b in zip(cache, held))
+    for name in ('norm_rotate', 'cache_append_rotated_', 'chunk_fwd'):
+        assert any(name in s for s in seen)
+
+
+def test_compiled_with_gradients():
+    q, k, v, wq, wk, cache, table, start, lengths, pos, rot, cu = _case()
+    dq, dk = (torch.randn_like(t) for t in (q, k))
+
+    def train(q, k, wq, wk):
+        y, z = kernels.norm_rotate(q * 2, k * 2, pos, rot, wq, wk, 1e-6)
+        return y + 1, z + 1
+
+    def step(fn):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, wq, wk)]
+        out = fn(*leaves)
+        return (*[t.detach() for t in out], *torch.autograd.grad(out, leaves, (dq, dk)))
+
+    got, want = step(torch.compile(train, backend='eager')), step(train)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
