@@ -25,6 +25,8 @@
 // iteration's chain and of its loads (9 tokens of 64 sequences of 4,096: 152 us, 3.6 TB/s, 2.3
 // us an iteration, of half of bf16's bytes, which takes 220 us, 4.9 TB/s; with codes asked for
 // two steps ahead, but no products among the softmax, as LDS has not room for both: 179 us).
+// A few rows over e4m3 are bound by latency too: the four tokens of eight sequences above, with
+// their join, take 26 us for 37 in bf16, 3.2 TB/s, with one tile a wave on its way in either type.
 // A workgroup takes one unit. Equal shares of all tiles' steps for as many workgroups as
 // are resident, tiles cut where a share ends, took longer (40 on 8 heads, 16 tokens of 48
 // sequences: 62 us for 53; four chunks of 512, head_dim 64: 162 for 131): starts and ends
@@ -184,7 +186,9 @@ __device__ __forceinline__ Unit unit_of_rank(const ChunkArgs& p, int rank, int l
   return x;
 }
 
-// More sequences: the tile of a slot, its splits side by side in the grid.
+// More sequences: the tile of a slot, its splits side by side in the grid, in the order given.
+// That ends with the longest sequence: 1 to 8,021 keys each, 4 tokens, 40 on 8 heads, 126
+// sequences by rank 123 us (e4m3 73), 127 by slot 201 (141), 256 287 (203).
 __device__ __forceinline__ Unit unit_of_slot(const ChunkArgs& p, int item, int lane) {
   Unit x;
   x.sp = span_of_slot(p.pk, false, p.n_slots - 1 - item / p.n_split, lane);

@@ -274,9 +274,10 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(RotateArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Gradients (24,960 tokens of 48 and 48 heads: 346 us, 5.3 TB/s of x, dy and dx, and 5 us
-// for the second launch). A wave's sums for the weights stay in its lanes' registers over all
-// of its tokens, and are joined over the lanes and waves of a workgroup, then over
+// Gradients (24,960 tokens of 48 and 48 heads: 337 us, 5.5 TB/s of x, dy and dx, and 5 us
+// for the second launch; a rotation without a norm 331, for x is read there too, which
+// it has no use for). A wave's sums for the weights stay in its lanes' registers over
+// all of its tokens, and are joined over the lanes and waves of a workgroup, then over
 // the workgroups by a second launch, in an order that the sizes alone set.
 
 struct RotateBwdArgs {
@@ -506,9 +507,9 @@ __global__ void __launch_bounds__(256) append_rotated_kernel(AppendRotatedArgs p
 }
 
 // Waves that fill the GPU; workgroups of a launch, which take their tokens in turn: many
-// where each stands alone (a clip of 57,720 tokens, four a workgroup at a time: 543 us
-// with 2,048, 523 with 16,384), few where each leaves sums (24,960 tokens and
-// gradients: 653, 593, 602 with 512, 768, 1,024).
+// where each stands alone (a clip of 57,720 tokens, four a workgroup at a time: 514, 508
+// and 496 us with 2,048, 4,096 and 16,384), few where each leaves sums (the gradients of
+// 24,960 tokens: 407, 342 and 345 with 512, 768 and 1,024).
 constexpr int64_t kEnough = 4096, kMostBlocks = 16384, kMostBwdBlocks = 768;
 
 // A launch's parts: waves for `rounds` rounds of every row, all by one where rows

@@ -337,9 +337,15 @@ def _chunk_splits(rows: int, heads: int, kv_heads: int, d: int, n_seq: int, capa
     most) of chunk_fwd. How many a sequence gets is up to the lengths, which are on the GPU;
     here are the room for it and the grid: splits of 256 keys at least, 128 MB of sums,
     and no more of them than the lengths can ask for where all are as long as the table
-    (sqrt(W R / (2 s)), with W steps of 64 keys on R places and s = 8)."""
+    (sqrt(W R / (2 s)), with W steps of 64 keys on R places and s = 8).
+
+    Beyond 126 sequences the kernel does not plan by lengths: a sequence's splits lie side
+    by side, as many as fill the GPU with all sequences alike, one from five key heads on.
+    So a long sequence is then walked by few workgroups: one of 32,768 positions beside
+    others of 200, four tokens, 32 heads on 8, takes 48 us with 126 sequences and 319 with
+    127."""
     room = min(-(-capacity // 256), _CHUNK_WORK // max(4 * rows * heads * (d + 2), 1), 64)
-    if n_seq > _CHUNK_RANKED:  # tiles enough for most; a sequence's splits lie side by side
+    if n_seq > _CHUNK_RANKED:
         room = min(room, -(-512 // (n_seq * kv_heads)))
     resident = max((512 if d == 128 else 768) // kv_heads, 1)
     tiles = rows * heads // kv_heads // TILE + min(n_seq, rows)

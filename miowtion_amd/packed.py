@@ -220,6 +220,11 @@ def paged_chunk_attention(q: torch.Tensor, cu: torch.Tensor, cache: PagedCache, 
 
     Rows that meet a NaN or an infinity in v that the mask hides within their tile are
     formed key by key, as packed_attention's. Without gradients, as the cache has none.
+
+    Work is shared out by the sequences' lengths for up to 126 of them. Beyond, a sequence
+    much longer than the others is what the call waits for (one of 32,768 positions beside
+    126 of 200, 8 key heads: 319 us, beside 125 of them 48): where lengths differ, batches
+    of up to 126 take less time.
     """
     res = ops_packed.chunk_fwd(q, cu, cache.k, cache.v, cache.k_exp, cache.v_exp, table, lengths, causal,
                                _scale(scale, q.shape[-1]), return_lse)
